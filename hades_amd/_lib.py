@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # constants); by default the in-tree build is used.
 LIB_PATH = os.environ.get("HADES_LIB_PATH") or os.path.join(_HERE, "csrc", "libhades_hip.so")
 
-F32, F64 = 0, 1
+F32, F64, F16, BF16 = 0, 1, 2, 3      # F16, BF16: the input-stage operators only
 I32, I64, I16, I8, U8 = 0, 1, 2, 3, 4
 COMBINE_FAST, COMBINE_EXACT = 0, 1
 HOST_NONCOHERENT = 1
@@ -21,12 +21,13 @@ COMBINE_STATIC_SCRATCH_BYTES = 16 << 20
 
 _P = c_void_p
 _L = c_int64
+_DROP = [ctypes.c_double, ctypes.c_uint64, _L, _P]      # p, seed, offset, offset_ptr
 
 # name -> argument types; every function returns int unless listed in _RESTYPE
 KERNEL_NONE, KERNEL_CACHED_FETCH, KERNEL_SEG_SUM, KERNEL_ADAGRAD, KERNEL_RADIX_PASS = 0, 1, 2, 3, 4
 KERNEL_HASH_ACCUMULATE = 5
 KERNEL_ADAM = 6
-ABI_VERSION = 131      # HADES_ABI_VERSION of include/hades_hip.h
+ABI_VERSION = 132      # HADES_ABI_VERSION of include/hades_hip.h
 
 _SIGNATURES = {
     "hades_profile_kernel": [c_int, _P, _P],
@@ -99,6 +100,13 @@ _SIGNATURES = {
     "hades_coldcache_accumulate": [_P, _P, _P, _L, _L, _L, _L, _P, _P, _P, _P, _P, _P],
     "hades_coldcache_flush": [_L, _L, c_int, _L, _P, _P, _P, _P, _P, _P, _P, _L, _P, _P, _P, _P,
                               _L, _P, c_size_t, _P],
+    "hades_embed": [_P, _L, _L, _P, _L, _P, _L, c_int, c_int, c_float, *_DROP, _P],
+    "hades_embed_grad": [_P, _L, _P, _L, _P, _L, _L, _L, c_int, c_int, c_int, _L, c_int, c_float, *_DROP, _P,
+                         c_size_t, _P],
+    "hades_dropout": [_P, _L, _P, _L, _P, _L, _L, c_int, *_DROP, _P],
+    "hades_rms_norm": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _L, _L, c_int, c_int, c_int, _L, c_float, *_DROP, _P],
+    "hades_rms_norm_grad": [_P, _L, _P, _L, _P, _P, _P, _L, _P, _P, _P, _L, _L, c_int, c_int, c_int, *_DROP, _P,
+                            c_size_t, _P],
 }
 _SIZE_QUERIES = {
     "hades_sort_mode": [],
@@ -112,6 +120,8 @@ _SIZE_QUERIES = {
     "hades_sacache_workspace_bytes": [_L],
     "hades_sacache_getall_workspace_bytes": [_L],
     "hades_coldcache_flush_workspace_bytes": [_L],
+    "hades_embed_grad_workspace_bytes": [_L, _L, _L],
+    "hades_rms_norm_grad_workspace_bytes": [_L, _L],
 }
 
 _lib = None

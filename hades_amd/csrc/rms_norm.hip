@@ -1,0 +1,620 @@
+// Root-mean-square norm of rows, with dropout and the residual's addition in front of it, an output
+// in 8 bits behind it, and its gradient.
+//
+//   h = residual + dropout(x)      rstd = 1 / sqrt(mean(h^2) + eps)      y = h * rstd * weight
+//   8 bits: for every row, or group of `group` columns, scale = max|y| / 448 and q = e4m3(y / scale)
+//
+//   with n = h * rstd and a = grad_y * weight:
+//   grad_residual = rstd * (a - n * mean(a * n)) + grad_h      grad_x = dropout(grad_residual)
+//   grad_weight   = sum over rows of grad_y * n
+//
+// All arithmetic is in float32; the norm is taken of the float32 h, which is rounded only where it is
+// stored.  Bound by memory: a row is read once and stays in registers between the sum over it and the
+// values made from it.  A row belongs to T lanes that hold K pieces of eight columns each, T from 8
+// lanes (rows of 64 columns) to 512 (16 384); longer rows are read again for each step.
+#include "rowvec.h"
+
+namespace hades {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kE4m3Max = 448.0f;
+constexpr int64_t kMaxPieces = 2048;   // of a row that stays in registers
+constexpr int64_t kMostThreads = int64_t(1) << 32;   // of a launch
+
+__device__ __forceinline__ f32x8 load8_as(const void* p, int64_t at, bool f32, int valid, const float*) {
+  (void)f32;
+  return load8(static_cast<const float*>(p) + at, valid);
+}
+// a tensor whose type is the rows' T, or float32
+template <typename T>
+__device__ __forceinline__ f32x8 load8_as(const void* p, int64_t at, bool f32, int valid, const T*) {
+  return f32 ? load8(static_cast<const float*>(p) + at, valid) : load8(static_cast<const T*>(p) + at, valid);
+}
+template <typename T>
+__device__ __forceinline__ void store8_as(void* p, int64_t at, bool f32, f32x8 v, int valid, const T*) {
+  if (f32) store8(static_cast<float*>(p) + at, v, valid);
+  else store8(static_cast<T*>(p) + at, v, valid);
+}
+
+__device__ __forceinline__ float sum8(f32x8 v) {
+  return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+}
+
+// Sum over the T lanes of a row; every lane gets it.  For T > 64 `shared` has T / 64 values and all
+// threads of the block call (T is the block's size then).
+template <int T>
+__device__ __forceinline__ float row_sum(float v, float* shared) {
+#pragma unroll
+  for (int d = 1; d < (T < kWave ? T : kWave); d <<= 1) v += __shfl_xor(v, d, kWave);
+  if (T > kWave) {
+    __syncthreads();   // `shared` may still be read for the value before
+    if ((threadIdx.x & (kWave - 1)) == 0) shared[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = shared[0];
+#pragma unroll
+    for (int w = 1; w < T / kWave; ++w) v += shared[w];
+  }
+  return v;
+}
+
+// Largest magnitude over groups of `lanes` lanes of a wave (a power of two), as bits: magnitudes
+// compare like whole numbers, and a NaN counts as larger than an infinity.
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v, int lanes) {
+  for (int d = 1; d < lanes; d <<= 1) {
+    const uint32_t o = __shfl_xor(v, d, kWave);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+
+__device__ __forceinline__ uint32_t max8(f32x8 v) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < kPiece; ++j) {
+    const uint32_t b = __float_as_uint(v[j]) & 0x7fffffffu;
+    m = b > m ? b : m;
+  }
+  return m;
+}
+
+// eight values in units of `scale`, rounded to e4m3 (nearest even); a group of zeros (scale 0) gives
+// zeros.  The division is the one of the definition: a product with 1 / scale could land on the other
+// side of a tie, and would overflow for the smallest scales.
+__device__ __forceinline__ void store_e4m3(uint8_t* __restrict__ p, f32x8 v, float scale, int valid) {
+  float u[kPiece];
+#pragma unroll
+  for (int j = 0; j < kPiece; ++j) {
+    const float r = scale > 0.0f ? v[j] / scale : 0.0f;
+    // (a NaN stays one: both comparisons are false)
+    u[j] = r > kE4m3Max ? kE4m3Max : (r < -kE4m3Max ? -kE4m3Max : r);
+  }
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(u[2], u[3], lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(u[4], u[5], hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(u[6], u[7], hi, true);
+  if (valid >= kPiece) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    typedef u32x2 u32x2u __attribute__((aligned(1)));
+    const u32x2 w = {static_cast<uint32_t>(lo), static_cast<uint32_t>(hi)};
+    *reinterpret_cast<u32x2u*>(p) = w;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < kPiece - 1; ++j)
+    if (j < valid) p[j] = static_cast<uint8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
+}
+
+// ---- forward ------------------------------------------------------------------------------------
+struct NormArgs {
+  const void* x;
+  const void* residual;   // may be null
+  const void* weight;     // may be null
+  void* y;                // rows' type, or e4m3 with `scales`
+  void* h;                // may be null
+  float* rstd;            // may be null
+  float* scales;
+  int64_t x_stride, res_stride, rows, cols;
+  int stream_f32, weight_f32;
+  int group_lanes;        // lanes that share a scale; 0: the row
+  int64_t groups;         // scales of a row
+  float eps;
+  DropArgs drop;
+};
+
+__device__ __forceinline__ int valid_of(int64_t cols, int64_t piece) {
+  const int64_t left = cols - piece * kPiece;
+  return left <= 0 ? 0 : (left < kPiece ? static_cast<int>(left) : kPiece);
+}
+
+template <typename X>
+__device__ __forceinline__ f32x8 load_h(const NormArgs& a, const DropKeys& keys, int64_t row, int64_t piece, int valid) {
+  const X* tag = nullptr;
+  f32x8 v = load8(static_cast<const X*>(a.x) + row * a.x_stride + piece * kPiece, valid);
+  f32x8 r;
+  if (a.residual != nullptr)
+    r = load8_as(a.residual, row * a.res_stride + piece * kPiece, a.stream_f32, valid, tag);
+  if (keys.on()) v = keys.apply(v, static_cast<uint32_t>(row), static_cast<uint32_t>(piece));
+  if (a.residual != nullptr) v += r;
+  return v;
+}
+
+template <typename X, int T, int K, bool kEight>
+__global__ __launch_bounds__(T > kThreads ? T : kThreads) void rms_norm_kernel(NormArgs a) {
+  constexpr int kRows = T > kThreads ? 1 : kThreads / T;
+  __shared__ float shared[T > kWave ? T / kWave : 1];
+  const X* tag = nullptr;
+  const DropKeys keys(a.drop);
+  const int lane = threadIdx.x % T;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / T;
+  const bool in = row < a.rows;
+  f32x8 h[K], w[K];
+  int valid[K];
+  float ss = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int64_t piece = k * T + lane;
+    valid[k] = in ? valid_of(a.cols, piece) : 0;
+    h[k] = load_h<X>(a, keys, row, piece, valid[k]);
+    if (a.weight != nullptr) w[k] = load8_as(a.weight, piece * kPiece, a.weight_f32, valid[k], tag);
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (a.h != nullptr)
+      store8_as(a.h, row * a.cols + (k * T + lane) * kPiece, a.stream_f32, h[k], valid[k], tag);
+    ss += sum8(h[k] * h[k]);
+  }
+  ss = row_sum<T>(ss, shared);
+  const float rstd = 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps);
+  if (a.rstd != nullptr && lane == 0 && in) a.rstd[row] = rstd;
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    h[k] *= rstd;
+    if (a.weight != nullptr) h[k] *= w[k];
+    if (!kEight) {
+      store8(static_cast<X*>(a.y) + row * a.cols + (k * T + lane) * kPiece, h[k], valid[k]);
+    } else if (a.group_lanes == 0) {
+      const uint32_t m = max8(h[k]);
+      top = m > top ? m : top;
+    }
+  }
+  if (!kEight) return;
+  if (a.group_lanes == 0) {
+    __shared__ uint32_t tops[T > kWave ? T / kWave : 1];
+    top = lanes_max(top, T < kWave ? T : kWave);
+    if (T > kWave) {
+      if ((threadIdx.x & (kWave - 1)) == 0) tops[threadIdx.x / kWave] = top;
+      __syncthreads();
+      top = tops[0];
+#pragma unroll
+      for (int i = 1; i < T / kWave; ++i) top = tops[i] > top ? tops[i] : top;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int piece = k * T + lane;
+    uint32_t m = top;
+    if (a.group_lanes != 0) m = lanes_max(max8(h[k]), a.group_lanes < T ? a.group_lanes : T);
+    const float scale = __uint_as_float(m) / kE4m3Max;
+    const bool first = a.group_lanes == 0 ? piece == 0 : (piece & (a.group_lanes - 1)) == 0;
+    if (first && valid[k] > 0) a.scales[row * a.groups + (a.group_lanes == 0 ? 0 : piece / a.group_lanes)] = scale;
+    store_e4m3(static_cast<uint8_t*>(a.y) + row * a.cols + static_cast<int64_t>(piece) * kPiece, h[k], scale, valid[k]);
+  }
+}
+
+// rows of more than kMaxPieces pieces: h is made again for each step
+template <typename X, bool kEight>
+__global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs a) {
+  constexpr int T = 1024;
+  __shared__ float shared[T / kWave];
+  __shared__ uint32_t tops[T / kWave];
+  const X* tag = nullptr;
+  const DropKeys keys(a.drop);
+  const int64_t row = blockIdx.x;
+  const int64_t pieces = (a.cols + kPiece - 1) / kPiece;
+  const int64_t rounds = (pieces + T - 1) / T;
+  float ss = 0.0f;
+  for (int64_t k = 0; k < rounds; ++k) {
+    const int64_t piece = k * T + threadIdx.x;
+    const int valid = valid_of(a.cols, piece);
+    const f32x8 h = load_h<X>(a, keys, row, piece, valid);
+    ss += sum8(h * h);
+  }
+  ss = row_sum<T>(ss, shared);
+  const float rstd = 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps);
+  if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = rstd;
+  uint32_t top = 0;
+  if (kEight && a.group_lanes == 0) {
+    for (int64_t k = 0; k < rounds; ++k) {
+      const int64_t piece = k * T + threadIdx.x;
+      const int valid = valid_of(a.cols, piece);
+      f32x8 y = load_h<X>(a, keys, row, piece, valid) * rstd;
+      if (a.weight != nullptr) y *= load8_as(a.weight, piece * kPiece, a.weight_f32, valid, tag);
+      const uint32_t m = max8(y);
+      top = m > top ? m : top;
+    }
+    top = lanes_max(top, kWave);
+    if ((threadIdx.x & (kWave - 1)) == 0) tops[threadIdx.x / kWave] = top;
+    __syncthreads();
+    for (int i = 0; i < T / kWave; ++i) top = tops[i] > top ? tops[i] : top;
+  }
+  for (int64_t k = 0; k < rounds; ++k) {
+    const int64_t piece = k * T + threadIdx.x;
+    const int valid = valid_of(a.cols, piece);
+    const int64_t at = row * a.cols + piece * kPiece;
+    f32x8 y = load_h<X>(a, keys, row, piece, valid);
+    if (a.h != nullptr) store8_as(a.h, at, a.stream_f32, y, valid, tag);
+    y *= rstd;
+    if (a.weight != nullptr) y *= load8_as(a.weight, piece * kPiece, a.weight_f32, valid, tag);
+    if (!kEight) {
+      store8(static_cast<X*>(a.y) + at, y, valid);
+      continue;
+    }
+    const uint32_t m = a.group_lanes != 0 ? lanes_max(max8(y), a.group_lanes) : top;
+    const float scale = __uint_as_float(m) / kE4m3Max;
+    const bool first = a.group_lanes == 0 ? piece == 0 : (piece & (a.group_lanes - 1)) == 0;
+    if (first && valid > 0) a.scales[row * a.groups + (a.group_lanes == 0 ? 0 : piece / a.group_lanes)] = scale;
+    store_e4m3(static_cast<uint8_t*>(a.y) + at, y, scale, valid);
+  }
+}
+
+// ---- gradient -----------------------------------------------------------------------------------
+struct NormGradArgs {
+  const void* grad;      // of y, rows' type
+  const void* h;         // the stream's type
+  const void* weight;    // may be null
+  const float* rstd;
+  const void* grad_h;    // may be null; the stream's type
+  void* grad_x;          // rows' type
+  void* grad_res;        // may be null; the stream's type
+  float* partial;        // [blocks][cols] rows of grad_weight's sum; null without grad_weight
+  int64_t grad_stride, h_stride, grad_h_stride, rows, cols;
+  int stream_f32, weight_f32;
+  DropArgs drop;
+};
+
+// A block takes every gridDim.x-th group of rows, so that a lane meets the same columns again and
+// keeps its part of grad_weight in registers until the end.
+template <typename X, int T, int K>
+__global__ __launch_bounds__(T > kThreads ? T : kThreads) void rms_norm_grad_kernel(NormGradArgs a) {
+  constexpr int kRows = T > kThreads ? 1 : kThreads / T;
+  __shared__ float shared[T > kWave ? T / kWave : 1];
+  __shared__ f32x8 parts[T < kThreads ? kThreads * K : 1];
+  const X* tag = nullptr;
+  const DropKeys keys(a.drop);
+  const int lane = threadIdx.x % T;
+  const int sub = threadIdx.x / T;
+  const float inv_cols = 1.0f / static_cast<float>(a.cols);
+  const f32x8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const f32x8 one = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+  f32x8 w[K], dw[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int64_t piece = k * T + lane;
+    dw[k] = zero;
+    w[k] = a.weight != nullptr ? load8_as(a.weight, piece * kPiece, a.weight_f32, valid_of(a.cols, piece), tag) : one;
+  }
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.rows; base += static_cast<int64_t>(gridDim.x) * kRows) {
+    const int64_t row = base + sub;
+    const bool in = row < a.rows;
+    const float rstd = in ? a.rstd[row] : 0.0f;
+    f32x8 g[K], n[K], gh[K];
+    int valid[K];
+    float dot = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t piece = k * T + lane;
+      valid[k] = in ? valid_of(a.cols, piece) : 0;
+      g[k] = load8(static_cast<const X*>(a.grad) + row * a.grad_stride + piece * kPiece, valid[k]);
+      n[k] = load8_as(a.h, row * a.h_stride + piece * kPiece, a.stream_f32, valid[k], tag);
+      if (a.grad_h != nullptr)
+        gh[k] = load8_as(a.grad_h, row * a.grad_h_stride + piece * kPiece, a.stream_f32, valid[k], tag);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      n[k] *= rstd;
+      dw[k] += g[k] * n[k];
+      g[k] *= w[k];
+      dot += sum8(g[k] * n[k]);
+    }
+    const float along = row_sum<T>(dot, shared) * inv_cols;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t piece = k * T + lane;
+      f32x8 d = (g[k] - n[k] * along) * rstd;
+      if (a.grad_h != nullptr) d += gh[k];
+      if (a.grad_res != nullptr)
+        store8_as(a.grad_res, row * a.cols + piece * kPiece, a.stream_f32, d, valid[k], tag);
+      if (keys.on()) d = keys.apply(d, static_cast<uint32_t>(row), static_cast<uint32_t>(piece));
+      store8(static_cast<X*>(a.grad_x) + row * a.cols + piece * kPiece, d, valid[k]);
+    }
+  }
+  if (a.partial == nullptr) return;
+  if (kRows > 1) {   // the rows of a block, in order
+#pragma unroll
+    for (int k = 0; k < K; ++k) parts[k * kThreads + threadIdx.x] = dw[k];
+    __syncthreads();
+    if (sub != 0) return;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      for (int s = 1; s < kRows; ++s) dw[k] += parts[k * kThreads + s * T + lane];
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int64_t piece = k * T + lane;
+    store8(a.partial + blockIdx.x * a.cols + piece * kPiece, dw[k], valid_of(a.cols, piece));
+  }
+}
+
+// rows of more than kMaxPieces pieces: the row is read again behind the sum
+template <typename X>
+__global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(NormGradArgs a) {
+  constexpr int T = 1024;
+  __shared__ float shared[T / kWave];
+  const X* tag = nullptr;
+  const DropKeys keys(a.drop);
+  const int64_t row = blockIdx.x;
+  const int64_t pieces = (a.cols + kPiece - 1) / kPiece;
+  const float rstd = a.rstd[row];
+  float dot = 0.0f;
+  for (int64_t piece = threadIdx.x; piece < pieces; piece += T) {
+    const int valid = valid_of(a.cols, piece);
+    f32x8 g = load8(static_cast<const X*>(a.grad) + row * a.grad_stride + piece * kPiece, valid);
+    if (a.weight != nullptr) g *= load8_as(a.weight, piece * kPiece, a.weight_f32, valid, tag);
+    dot += sum8(g * (load8_as(a.h, row * a.h_stride + piece * kPiece, a.stream_f32, valid, tag) * rstd));
+  }
+  const float along = row_sum<T>(dot, shared) / static_cast<float>(a.cols);
+  for (int64_t piece = threadIdx.x; piece < pieces; piece += T) {
+    const int valid = valid_of(a.cols, piece);
+    f32x8 g = load8(static_cast<const X*>(a.grad) + row * a.grad_stride + piece * kPiece, valid);
+    if (a.weight != nullptr) g *= load8_as(a.weight, piece * kPiece, a.weight_f32, valid, tag);
+    const f32x8 n = load8_as(a.h, row * a.h_stride + piece * kPiece, a.stream_f32, valid, tag) * rstd;
+    f32x8 d = (g - n * along) * rstd;
+    if (a.grad_h != nullptr) d += load8_as(a.grad_h, row * a.grad_h_stride + piece * kPiece, a.stream_f32, valid, tag);
+    if (a.grad_res != nullptr) store8_as(a.grad_res, row * a.cols + piece * kPiece, a.stream_f32, d, valid, tag);
+    if (keys.on()) d = keys.apply(d, static_cast<uint32_t>(row), static_cast<uint32_t>(piece));
+    store8(static_cast<X*>(a.grad_x) + row * a.cols + piece * kPiece, d, valid);
+  }
+}
+
+// ... and grad_weight's partial rows: block (x, y) takes kThreads pieces and every gridDim.y-th row
+template <typename X>
+__global__ __launch_bounds__(kThreads) void rms_norm_grad_weight_kernel(NormGradArgs a) {
+  const X* tag = nullptr;
+  const int64_t piece = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int valid = valid_of(a.cols, piece);
+  if (valid == 0) return;
+  f32x8 dw = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const f32x8 g = load8(static_cast<const X*>(a.grad) + row * a.grad_stride + piece * kPiece, valid);
+    dw += g * (load8_as(a.h, row * a.h_stride + piece * kPiece, a.stream_f32, valid, tag) * a.rstd[row]);
+  }
+  store8(a.partial + blockIdx.y * a.cols + piece * kPiece, dw, valid);
+}
+
+// out[c] = sum of partial[0 .. blocks)[c]: 64 columns a block, 16 waves that take the rows in turn
+constexpr int kFoldWaves = 16;
+template <typename W>
+__global__ __launch_bounds__(kFoldWaves* kWave) void fold_rows_kernel(const float* __restrict__ partial, int64_t blocks,
+                                                                      int64_t cols, W* __restrict__ out) {
+  constexpr int U = 8;
+  __shared__ float part[kFoldWaves][kWave];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kWave + lane;
+  float acc = 0.0f;
+  if (col < cols) {
+    for (int64_t b = wave; b < blocks; b += kFoldWaves * U) {
+      float v[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int64_t i = b + k * kFoldWaves;
+        v[k] = i < blocks ? partial[i * cols + col] : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) acc += v[k];
+    }
+  }
+  part[wave][lane] = acc;
+  __syncthreads();
+  if (wave != 0 || col >= cols) return;
+  for (int w = 1; w < kFoldWaves; ++w) acc += part[w][lane];
+  out[col] = static_cast<W>(acc);
+}
+
+template <typename X, bool kEight>
+int launch_norm(const NormArgs& a, hipStream_t st) {
+  const int64_t pieces = ceil_div(a.cols, kPiece);
+  if (pieces > kMaxPieces) {
+    HADES_REQUIRE(a.rows < kMostThreads / 1024, "rms_norm: too many rows for one call");
+    HADES_LAUNCH((rms_norm_long_kernel<X, kEight>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st, a);
+    return HADES_OK;
+  }
+#define HADES_NORM(T_, K_)                                                                              \
+  do {                                                                                                  \
+    constexpr int kBlock = T_ > kThreads ? T_ : kThreads;                                               \
+    const int64_t blocks = ceil_div(a.rows, kBlock / T_);                                               \
+    HADES_REQUIRE(blocks < kMostThreads / kBlock, "rms_norm: too many rows for one call");              \
+    HADES_LAUNCH((rms_norm_kernel<X, T_, K_, kEight>), dim3(static_cast<unsigned>(blocks)),             \
+                 dim3(kBlock), 0, st, a);                                                               \
+    return HADES_OK;                                                                                    \
+  } while (0)
+  if (pieces <= 8) HADES_NORM(8, 1);
+  if (pieces <= 16) HADES_NORM(16, 1);
+  if (pieces <= 32) HADES_NORM(32, 1);
+  if (pieces <= 64) HADES_NORM(64, 1);
+  if (pieces <= 128) HADES_NORM(64, 2);
+  if (pieces <= 256) HADES_NORM(256, 1);
+  if (pieces <= 512) HADES_NORM(256, 2);
+  if (pieces <= 1024) HADES_NORM(256, 4);
+  HADES_NORM(512, 4);
+#undef HADES_NORM
+}
+
+// blocks of the gradient kernel: rows of grad_weight's partial sum
+constexpr int64_t kGradBlocks = 1024;
+
+int lanes_of(int64_t pieces) {
+  if (pieces > kMaxPieces) return 0;
+  if (pieces > 1024) return 512;
+  if (pieces > 128) return 256;
+  int t = 8;
+  while (t < kWave && t < pieces) t *= 2;
+  return t;
+}
+
+int64_t grad_blocks(int64_t rows, int64_t cols) {
+  const int t = lanes_of(ceil_div(cols, kPiece));
+  const int64_t blocks = t == 0 ? rows : ceil_div(rows, t >= kThreads ? 1 : kThreads / t);
+  const int64_t most = t == 0 ? 64 : kGradBlocks;
+  return blocks < most ? blocks : most;
+}
+
+template <typename X>
+int launch_norm_grad(const NormGradArgs& a, hipStream_t st) {
+  const int64_t pieces = ceil_div(a.cols, kPiece);
+  const unsigned blocks = static_cast<unsigned>(grad_blocks(a.rows, a.cols));
+  if (pieces > kMaxPieces) {
+    HADES_REQUIRE(a.rows < kMostThreads / 1024, "rms_norm_grad: too many rows for one call");
+    HADES_LAUNCH((rms_norm_grad_long_kernel<X>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st, a);
+    if (a.partial != nullptr)
+      HADES_LAUNCH((rms_norm_grad_weight_kernel<X>), dim3(static_cast<unsigned>(ceil_div(pieces, kThreads)), blocks),
+                   dim3(kThreads), 0, st, a);
+    return HADES_OK;
+  }
+#define HADES_NORM_GRAD(T_, K_)                                                                          \
+  do {                                                                                                   \
+    HADES_LAUNCH((rms_norm_grad_kernel<X, T_, K_>), dim3(blocks), dim3(T_ > kThreads ? T_ : kThreads),   \
+                 0, st, a);                                                                              \
+    return HADES_OK;                                                                                     \
+  } while (0)
+  if (pieces <= 8) HADES_NORM_GRAD(8, 1);
+  if (pieces <= 16) HADES_NORM_GRAD(16, 1);
+  if (pieces <= 32) HADES_NORM_GRAD(32, 1);
+  if (pieces <= 64) HADES_NORM_GRAD(64, 1);
+  if (pieces <= 128) HADES_NORM_GRAD(64, 2);
+  if (pieces <= 256) HADES_NORM_GRAD(256, 1);
+  if (pieces <= 512) HADES_NORM_GRAD(256, 2);
+  if (pieces <= 1024) HADES_NORM_GRAD(256, 4);
+  HADES_NORM_GRAD(512, 4);
+#undef HADES_NORM_GRAD
+}
+
+bool row_type(int dtype) { return dtype == HADES_F32 || dtype == HADES_F16 || dtype == HADES_BF16; }
+
+}  // namespace
+}  // namespace hades
+
+using namespace hades;
+
+extern "C" {
+
+int hades_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t res_stride, const void* weight,
+                   void* y, float* scales, void* h, float* rstd, int64_t rows, int64_t cols, int dtype,
+                   int stream_dtype, int weight_dtype, int64_t group, float eps, double p, uint64_t seed,
+                   int64_t offset, const int64_t* offset_ptr, void* stream) {
+  HADES_REQUIRE(rows >= 0 && cols >= 1, "rows must be >= 0 and cols >= 1");
+  HADES_REQUIRE(rows < (int64_t(1) << 32) && cols < (int64_t(1) << 31), "rms_norm: rows or cols too large");
+  HADES_REQUIRE(row_type(dtype), "Type can only be float, half or bfloat16");
+  HADES_REQUIRE(stream_dtype == dtype || stream_dtype == HADES_F32, "the residual's type is the rows' or float");
+  HADES_REQUIRE(weight_dtype == dtype || weight_dtype == HADES_F32, "the weight's type is the rows' or float");
+  HADES_REQUIRE(eps >= 0.0f, "eps must be >= 0");
+  HADES_REQUIRE(group == 0 || (is_pow2(group) && group >= kPiece && group <= kPiece * kWave),
+                "group must be 0 or a power of two in [8, 512]");
+  DropArgs drop;
+  HADES_REQUIRE(make_drop(p, seed, offset, offset_ptr, 1.0, &drop), "p must lie in [0, 1]");
+  if (rows == 0) return HADES_OK;
+  HADES_REQUIRE(x && y, "null pointer argument");
+  HADES_REQUIRE(x_stride >= cols || rows == 1, "row stride below cols");
+  HADES_REQUIRE(!residual || res_stride >= cols || rows == 1, "row stride below cols");
+  NormArgs a;
+  a.x = x;
+  a.residual = residual;
+  a.weight = weight;
+  a.y = y;
+  a.h = h;
+  a.rstd = rstd;
+  a.scales = scales;
+  a.x_stride = x_stride;
+  a.res_stride = res_stride;
+  a.rows = rows;
+  a.cols = cols;
+  a.stream_f32 = stream_dtype == HADES_F32;
+  a.weight_f32 = weight_dtype == HADES_F32;
+  a.group_lanes = static_cast<int>(group / kPiece);
+  a.groups = group == 0 ? 1 : ceil_div(cols, group);
+  a.eps = eps;
+  a.drop = drop;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+#define HADES_NORM_TYPE(X_) return scales != nullptr ? launch_norm<X_, true>(a, st) : launch_norm<X_, false>(a, st)
+  if (dtype == HADES_F32) HADES_NORM_TYPE(float);
+  if (dtype == HADES_F16) HADES_NORM_TYPE(f16);
+  HADES_NORM_TYPE(bf16);
+#undef HADES_NORM_TYPE
+}
+
+size_t hades_rms_norm_grad_workspace_bytes(int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 1) return 0;
+  const size_t b = static_cast<size_t>(grad_blocks(rows > 0 ? rows : 1, cols)) * cols * sizeof(float);
+  return (b + 255) & ~size_t(255);
+}
+
+int hades_rms_norm_grad(const void* grad, int64_t grad_stride, const void* h, int64_t h_stride, const void* weight,
+                        const float* rstd, const void* grad_h, int64_t grad_h_stride, void* grad_x, void* grad_res,
+                        void* grad_weight, int64_t rows, int64_t cols, int dtype, int stream_dtype,
+                        int weight_dtype, double p, uint64_t seed, int64_t offset, const int64_t* offset_ptr,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  HADES_REQUIRE(rows >= 0 && cols >= 1, "rows must be >= 0 and cols >= 1");
+  HADES_REQUIRE(rows < (int64_t(1) << 32) && cols < (int64_t(1) << 31), "rms_norm_grad: rows or cols too large");
+  HADES_REQUIRE(row_type(dtype), "Type can only be float, half or bfloat16");
+  HADES_REQUIRE(stream_dtype == dtype || stream_dtype == HADES_F32, "the residual's type is the rows' or float");
+  HADES_REQUIRE(weight_dtype == dtype || weight_dtype == HADES_F32, "the weight's type is the rows' or float");
+  HADES_REQUIRE(!grad_weight || weight, "grad_weight without a weight");
+  DropArgs drop;
+  HADES_REQUIRE(make_drop(p, seed, offset, offset_ptr, 1.0, &drop), "p must lie in [0, 1]");
+  if (rows == 0 && !grad_weight) return HADES_OK;
+  HADES_REQUIRE(rows == 0 || (grad && h && rstd && grad_x), "null pointer argument");
+  HADES_REQUIRE(grad_stride >= cols || rows <= 1, "row stride below cols");
+  HADES_REQUIRE(h_stride >= cols || rows <= 1, "row stride below cols");
+  HADES_REQUIRE(!grad_h || grad_h_stride >= cols || rows <= 1, "row stride below cols");
+  const size_t need = hades_rms_norm_grad_workspace_bytes(rows, cols);
+  if (grad_weight && (workspace == nullptr || workspace_bytes < need))
+    return set_error(HADES_ERR_WORKSPACE, "rms_norm_grad workspace too small: need %zu bytes, got %zu", need,
+                     workspace_bytes);
+  HADES_REQUIRE((align_of_ptr(workspace) & 255) == 0, "workspace must be 256-byte aligned");
+  NormGradArgs a;
+  a.grad = grad;
+  a.h = h;
+  a.weight = weight;
+  a.rstd = rstd;
+  a.grad_h = grad_h;
+  a.grad_x = grad_x;
+  a.grad_res = grad_res;
+  a.partial = grad_weight ? static_cast<float*>(workspace) : nullptr;
+  a.grad_stride = grad_stride;
+  a.h_stride = h_stride;
+  a.grad_h_stride = grad_h_stride;
+  a.rows = rows;
+  a.cols = cols;
+  a.stream_f32 = stream_dtype == HADES_F32;
+  a.weight_f32 = weight_dtype == HADES_F32;
+  a.drop = drop;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  int rc = HADES_OK;
+  if (rows > 0)
+    rc = dtype == HADES_F32 ? launch_norm_grad<float>(a, st)
+                            : (dtype == HADES_F16 ? launch_norm_grad<f16>(a, st) : launch_norm_grad<bf16>(a, st));
+  if (rc != HADES_OK || !grad_weight) return rc;
+  const int64_t blocks = rows > 0 ? grad_blocks(rows, cols) : 0;
+  const dim3 grid(static_cast<unsigned>(ceil_div(cols, kWave))), block(kFoldWaves * kWave);
+#define HADES_FOLD(W_) \
+  HADES_LAUNCH((fold_rows_kernel<W_>), grid, block, 0, st, a.partial, blocks, cols, static_cast<W_*>(grad_weight))
+  if (weight_dtype == HADES_F32) HADES_FOLD(float);
+  else if (weight_dtype == HADES_F16) HADES_FOLD(f16);
+  else HADES_FOLD(bf16);
+#undef HADES_FOLD
+  return HADES_OK;
+}
+
+}  // extern "C"

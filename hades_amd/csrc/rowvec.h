@@ -1,0 +1,136 @@
+// Rows of float32 / float16 / bfloat16 in pieces of eight values, and the counter-based generator
+// behind dropout.  Shared by embed.hip, dropout.hip and rms_norm.hip (not part of the C ABI).
+#pragma once
+
+#include "common.h"
+
+namespace hades {
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+
+// eight values of a row: one 16-byte access for the 16-bit types, two for float32
+constexpr int kPiece = 8;
+
+// ---- dropout's arguments ------------------------------------------------------------------------
+// p as a whole number of 65536ths (0: nothing dropped), the factor of the kept values, and the
+// generator's key and counter.  offset_ptr (device, may be null) is added to offset when the kernel
+// runs, so that a replayed graph can draw other numbers each time.
+struct DropArgs {
+  uint32_t threshold;
+  float factor;
+  uint32_t key0, key1;
+  uint64_t offset;
+  const int64_t* offset_ptr;
+};
+
+// p in [0, 1] to DropArgs; `scale` is a further factor of the kept values.
+inline bool make_drop(double p, uint64_t seed, int64_t offset, const int64_t* offset_ptr, double scale,
+                      DropArgs* d) {
+  if (!(p >= 0.0 && p <= 1.0)) return false;
+  d->threshold = static_cast<uint32_t>(p * 65536.0 + 0.5);
+  d->factor = d->threshold >= 65536u
+                  ? 0.0f : static_cast<float>(scale * (65536.0 / (65536.0 - d->threshold)));
+  d->key0 = static_cast<uint32_t>(seed);
+  d->key1 = static_cast<uint32_t>(seed >> 32);
+  d->offset = static_cast<uint64_t>(offset);
+  d->offset_ptr = offset_ptr;
+  return true;
+}
+
+// n / d for n < 2^31 as a multiplication (Granlund and Montgomery's round-up form)
+struct FastDiv {
+  uint32_t d, mul, shift;
+  explicit FastDiv(uint32_t div = 1) : d(div) {
+    shift = static_cast<uint32_t>(ilog2_ceil(div));
+    mul = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - div)) / div + 1);
+  }
+#if defined(__HIPCC__)
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+#endif
+};
+
+#if defined(__HIPCC__)
+
+template <typename T>
+struct Vec8 {
+  typedef T V __attribute__((ext_vector_type(8)));
+  // a row may start at any element: the access is only as aligned as one value (gfx950 serves
+  // unaligned wide accesses, a row of odd width takes the same instructions as any other)
+  typedef V VU __attribute__((aligned(sizeof(T))));
+};
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// p[0 .. 8) (or its first `valid` values, zeros behind them) as float32
+template <typename T, bool kOnce = false>
+__device__ __forceinline__ f32x8 load8(const T* __restrict__ p, int valid) {
+  if (valid >= kPiece) {
+    typedef typename Vec8<T>::VU VU;
+    const VU v = kOnce ? __builtin_nontemporal_load(reinterpret_cast<const VU*>(p))
+                       : *reinterpret_cast<const VU*>(p);
+    return __builtin_convertvector(v, f32x8);
+  }
+  f32x8 r = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < kPiece - 1; ++j)
+    if (j < valid) r[j] = static_cast<float>(p[j]);
+  return r;
+}
+
+// rounds to nearest even, once
+template <typename T>
+__device__ __forceinline__ void store8(T* __restrict__ p, f32x8 v, int valid) {
+  if (valid >= kPiece) {
+    typedef typename Vec8<T>::V V;
+    typedef typename Vec8<T>::VU VU;
+    *reinterpret_cast<VU*>(p) = __builtin_convertvector(v, V);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < kPiece - 1; ++j)
+    if (j < valid) p[j] = static_cast<T>(v[j]);
+}
+
+// Philox4x32 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", 2011) with
+// seven rounds, the fewest that pass the paper's statistical tests: 128 bits for eight values of a row.
+// Per piece 14 products of 32 x 32 bits; a dropout of bfloat16 rows stays bound by memory.
+struct DropKeys {
+  uint32_t threshold, key0, key1, off0, off1;
+  float factor;
+  __device__ __forceinline__ explicit DropKeys(const DropArgs& d)
+      : threshold(d.threshold), key0(d.key0), key1(d.key1), factor(d.factor) {
+    uint64_t o = d.offset;
+    if (d.offset_ptr != nullptr) o += static_cast<uint64_t>(*d.offset_ptr);
+    off0 = static_cast<uint32_t>(o);
+    off1 = static_cast<uint32_t>(o >> 32);
+  }
+  __device__ __forceinline__ bool on() const { return threshold != 0u; }
+
+  // keeps or zeroes the eight values of piece `piece` of row `row`; kept ones are multiplied by
+  // factor.  A value that is dropped is 0 whatever it was, infinities and NaN too.
+  __device__ __forceinline__ f32x8 apply(f32x8 v, uint32_t row, uint32_t piece) const {
+    uint32_t c0 = piece, c1 = row, c2 = off0, c3 = off1, k0 = key0, k1 = key1;
+#pragma unroll
+    for (int r = 0; r < 7; ++r) {
+      const uint64_t a = static_cast<uint64_t>(c0) * 0xD2511F53u;
+      const uint64_t b = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
+      c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
+      c1 = static_cast<uint32_t>(b);
+      c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
+      c3 = static_cast<uint32_t>(a);
+      k0 += 0x9E3779B9u;
+      k1 += 0xBB67AE85u;
+    }
+    const uint32_t w[4] = {c0, c1, c2, c3};
+#pragma unroll
+    for (int j = 0; j < kPiece; ++j) {
+      const uint32_t bits = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu;
+      v[j] = bits >= threshold ? v[j] * factor : 0.0f;
+    }
+    return v;
+  }
+};
+
+#endif  // __HIPCC__
+
+}  // namespace hades

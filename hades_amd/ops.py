@@ -837,3 +837,238 @@ def bucket_by_owner(ids, grad=None, cnt=None, partition_range=None, local_num_gp
     if return_perm:
         return ids_out, grad_out, cnt_out, split_sizes, perm
     return ids_out, grad_out, cnt_out, split_sizes
+
+
+# ---- input stage of a model: embedding with scaling, dropout, norm ------------------
+# Types float32, float16 and bfloat16, arithmetic in float32, one rounding where a value is stored.
+# The last dimension of a tensor is its row; rows may lie any distance apart, their values are
+# contiguous.  `dropout` = (p, seed, offset) names a mask that is drawn where it is needed and never
+# stored: value (row, column) is a function of the three and of its row and column alone.  p counts in
+# 65536ths (to the nearest), seed is any 64-bit number, offset an int or an int64 tensor of one element
+# on the device, read when the kernel runs (a captured step that adds to it draws new masks on replay).
+# Two calls of one step need different offsets, or their masks are equal.
+_ROW_TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_ID_TYPES = {torch.int32: _lib.I32, torch.int64: _lib.I64}
+_U64 = (1 << 64) - 1
+
+
+def _row_type(t, name):
+    code = _ROW_TYPES.get(t.dtype)
+    _check(code is not None, "Type can only be float, half or bfloat16 (%s is %s)" % (name, t.dtype))
+    return code
+
+
+def _row_stride(t, name, device):
+    """Elements between the rows of t (its last dimension), which lies on `device`."""
+    _check(t.is_cuda and t.device == device, "%s must be a device tensor on %s" % (name, device))
+    _check(t.dim() >= 1, "%s must have at least one dimension" % name)
+    cols = t.size(-1)
+    if t.is_contiguous() or t.numel() == 0:
+        return cols
+    try:
+        v = t.view(-1, cols)
+    except RuntimeError:
+        v = None
+    _check(v is not None and (cols == 1 or v.stride(1) == 1) and (v.size(0) == 1 or v.stride(0) >= cols),
+           "%s: rows must be contiguous, the same distance apart, and must not overlap" % name)
+    return v.stride(0) if v.size(0) > 1 else cols
+
+
+def _current(t, name):
+    _check(t.is_cuda, "%s must be a device tensor" % name)
+    _check(t.device.index == torch.cuda.current_device(),
+           "%s is on %s, which is not the current device: launches go to the current device's stream"
+           % (name, t.device))
+    return t.device
+
+
+def _drop_args(dropout, device):
+    if dropout is None:
+        return 0.0, 0, 0, _NULL
+    p, seed, offset = dropout
+    _check(0.0 <= p <= 1.0, "dropout: p must lie in [0, 1]")
+    ptr = _NULL
+    if isinstance(offset, torch.Tensor):
+        _check(offset.dtype == torch.int64 and offset.numel() == 1 and offset.device == device,
+               "dropout: offset must be an int or an int64 tensor of one element on the device")
+        ptr, offset = _ptr(offset), 0
+    _check(-(1 << 63) <= seed <= _U64 and 0 <= offset < (1 << 63),
+           "dropout: seed must fit 64 bits, offset must be in [0, 2^63)")
+    return float(p), seed & _U64, offset, ptr
+
+
+def _dense_out(out, shape, dtype, device, name="out"):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _check(out.device == device and out.is_contiguous(), "%s must be a contiguous tensor on %s" % (name, device))
+    _check(tuple(out.shape) == tuple(shape) and out.dtype == dtype, "%s has the wrong shape/dtype" % name)
+    return out
+
+
+def embed(weight, ids, scale=1.0, dropout=None, out=None):
+    """out[..., :] = scale * weight[ids[...], :], then dropout; rows of the table's type, of shape
+    ids.shape + (dim,).  weight [num_rows, dim] may be a row-strided view; ids int32 or int64.  An
+    id outside [0, num_rows) (padding, e.g. -1) gives a row of zeros."""
+    dev = _current(weight, "weight")
+    _check(weight.dim() == 2 and weight.size(1) >= 1, "weight must be [num_rows, dim]")
+    dtype, stride = _row_type(weight, "weight"), _row_stride(weight, "weight", dev)
+    itype = _ID_TYPES.get(ids.dtype)
+    _check(itype is not None, "ID can only be int32 or int64 (ids is %s)" % ids.dtype)
+    _check(ids.device == dev and ids.is_contiguous(), "ids must be a contiguous tensor on %s" % dev)
+    drop = _drop_args(dropout, dev)
+    dim = weight.size(1)
+    out = _dense_out(out, (*ids.shape, dim), weight.dtype, dev)
+    _lib.call("hades_embed", _ptr(weight), stride, weight.size(0), _ptr(ids), ids.numel(), _ptr(out), dim, dtype,
+              itype, float(scale), *drop, _stream())
+    return out
+
+
+def embed_grad(grad, ids, num_rows, scale=1.0, padding_idx=None, dropout=None, out=None, accumulate=False,
+               out_dtype=None):
+    """The gradient of embed's weight, dense: out[v, :] = scale * sum of dropout(grad) over the positions
+    that hold token v, with the sums in float32 in an order that (shape, ids) fix - the same bits on every
+    run.  Tokens that do not occur get rows of zeros.  `accumulate` adds to `out` instead and leaves the
+    rows of absent tokens alone.  Ids outside [0, num_rows) and `padding_idx` have no gradient.  `out`
+    ([num_rows, dim], may be row-strided) has grad's type or float32, as has `out_dtype`."""
+    dev = _current(grad, "grad")
+    dtype, stride = _row_type(grad, "grad"), _row_stride(grad, "grad", dev)
+    dim, n = grad.size(-1), ids.numel()
+    itype = _ID_TYPES.get(ids.dtype)
+    _check(itype is not None, "ID can only be int32 or int64 (ids is %s)" % ids.dtype)
+    _check(ids.device == dev and ids.is_contiguous(), "ids must be a contiguous tensor on %s" % dev)
+    _check(dim >= 1 and grad.numel() == n * dim, "grad must have one row per id")
+    _check(num_rows >= 0, "num_rows must be >= 0")
+    _check(padding_idx is None or 0 <= padding_idx < num_rows, "padding_idx must be in [0, num_rows)")
+    drop = _drop_args(dropout, dev)
+    if out is None:
+        _check(not accumulate, "accumulate needs out")
+        out = torch.empty((num_rows, dim), dtype=out_dtype or grad.dtype, device=dev)
+    _check(out.dim() == 2 and tuple(out.shape) == (num_rows, dim) and out_dtype in (None, out.dtype),
+           "out has the wrong shape/dtype")
+    _check(out.dtype in (grad.dtype, torch.float32), "the gradient's type is the rows' or float")
+    ws = torch.empty(_lib.query("hades_embed_grad_workspace_bytes", n, dim, num_rows), dtype=torch.uint8, device=dev)
+    _lib.call("hades_embed_grad", _ptr(grad), stride, _ptr(ids), n, _ptr(out), _row_stride(out, "out", dev), num_rows,
+              dim, dtype, _ROW_TYPES[out.dtype], itype, -1 if padding_idx is None else int(padding_idx),
+              int(bool(accumulate)), float(scale), *drop, _ptr(ws), ws.numel(), _stream())
+    return out
+
+
+def dropout(x, p, seed, offset, residual=None, out=None):
+    """out = x with a share p of its values zeroed and the others divided by 1 - p, plus `residual` (of
+    x's shape and type).  `out` may be x or residual."""
+    dev = _current(x, "x")
+    dtype, stride = _row_type(x, "x"), _row_stride(x, "x", dev)
+    res_stride = 0
+    if residual is not None:
+        _check(residual.shape == x.shape and residual.dtype == x.dtype, "residual must have x's shape and dtype")
+        res_stride = _row_stride(residual, "residual", dev)
+    drop = _drop_args((p, seed, offset), dev)
+    out = _dense_out(out, x.shape, x.dtype, dev)
+    if out.numel():
+        cols = x.size(-1)
+        _lib.call("hades_dropout", _ptr(x), stride, _opt(residual), res_stride, _ptr(out), x.numel() // cols, cols,
+                  dtype, *drop, _stream())
+    return out
+
+
+def dropout_grad(grad, p, seed, offset, out=None):
+    """The gradient of dropout's x (residual's gradient is grad itself): the mask of (p, seed, offset),
+    drawn again, on grad."""
+    return dropout(grad, p, seed, offset, out=out)
+
+
+def _norm_args(x, weight, residual, dropout, dev):
+    dtype = _row_type(x, "x")
+    _check(x.dim() >= 1 and x.size(-1) >= 1, "x must have rows of at least one value")
+    stream_type, res_stride, weight_type = x.dtype, 0, dtype
+    if residual is not None:
+        _check(residual.shape == x.shape and residual.dtype in (x.dtype, torch.float32),
+               "residual must have x's shape, and x's dtype or float32")
+        stream_type, res_stride = residual.dtype, _row_stride(residual, "residual", dev)
+    if weight is not None:
+        _check(weight.device == dev and tuple(weight.shape) == (x.size(-1),) and weight.is_contiguous()
+               and weight.dtype in (x.dtype, torch.float32),
+               "weight must be contiguous [columns of x] on %s, of x's dtype or float32" % dev)
+        weight_type = _ROW_TYPES[weight.dtype]
+    return dtype, stream_type, res_stride, weight_type, _drop_args(dropout, dev)
+
+
+def rms_norm(x, weight=None, eps=1e-6, residual=None, dropout=None, out=None, h_out=None):
+    """h = residual + dropout(x);  y = h / sqrt(mean(h^2) + eps) * weight over the last dimension.
+    Returns (y, h, rstd): y of x's type, h of the residual's (x itself where there is neither residual
+    nor dropout), rstd = 1 / sqrt(...) float32 of shape x.shape[:-1], for rms_norm_grad.  The norm is
+    taken of h before its rounding.  residual and weight have x's type or float32; weight None: ones.
+    `h_out` may be residual."""
+    dev = _current(x, "x")
+    dtype, stream_type, res_stride, weight_type, drop = _norm_args(x, weight, residual, dropout, dev)
+    stride, cols = _row_stride(x, "x", dev), x.size(-1)
+    y = _dense_out(out, x.shape, x.dtype, dev)
+    h = x
+    if residual is not None or dropout is not None or h_out is not None:
+        h = _dense_out(h_out, x.shape, stream_type, dev, "h_out")
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    _lib.call("hades_rms_norm", _ptr(x), stride, _opt(residual), res_stride, _opt(weight), _ptr(y), _NULL,
+              _NULL if h is x else _ptr(h), _ptr(rstd), rstd.numel(), cols, dtype, _ROW_TYPES[stream_type],
+              weight_type, 0, float(eps), *drop, _stream())
+    return y, h, rstd
+
+
+def rms_norm_8bit(x, weight=None, eps=1e-6, residual=None, group=0, dropout=None, h_out=None):
+    """rms_norm with y in 8 bits: (q float8_e4m3fn of x's shape, scales float32 x.shape[:-1] + (groups,),
+    h).  y is about q * scale, with one scale for every `group` columns (a power of two from 8 to 512; 0:
+    one for the row), scale = max|y| / 448.  A group of zeros has scale 0; one with an infinity or a NaN
+    has a scale that is one too."""
+    dev = _current(x, "x")
+    dtype, stream_type, res_stride, weight_type, drop = _norm_args(x, weight, residual, dropout, dev)
+    stride, cols = _row_stride(x, "x", dev), x.size(-1)
+    _check(group == 0 or (8 <= group <= 512 and group & (group - 1) == 0),
+           "group must be 0 or a power of two in [8, 512]")
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    groups = 1 if group == 0 else -(-cols // group)
+    scales = torch.empty((*x.shape[:-1], groups), dtype=torch.float32, device=dev)
+    h = x
+    if residual is not None or dropout is not None or h_out is not None:
+        h = _dense_out(h_out, x.shape, stream_type, dev, "h_out")
+    _lib.call("hades_rms_norm", _ptr(x), stride, _opt(residual), res_stride, _opt(weight), _ptr(q), _ptr(scales),
+              _NULL if h is x else _ptr(h), _NULL, scales.numel() // groups, cols, dtype, _ROW_TYPES[stream_type],
+              weight_type, int(group), float(eps), *drop, _stream())
+    return q, scales, h
+
+
+def rms_norm_grad(grad, h, weight, rstd, grad_h=None, dropout=None, weight_grad=True, residual_grad=True):
+    """The gradient of rms_norm from its h and rstd: (grad_x, grad_residual, grad_weight).  grad is y's
+    gradient, grad_h (h's type) the one that reaches h from elsewhere, or None.  grad_x has grad's type,
+    grad_residual h's; where the two have the same values and type they are one tensor.  grad_weight
+    (weight's type, summed in float32 in a fixed order) is None without weight or weight_grad,
+    grad_residual None without residual_grad."""
+    dev = _current(grad, "grad")
+    dtype = _row_type(grad, "grad")
+    _check(grad.dim() >= 1 and grad.size(-1) >= 1, "grad must have rows of at least one value")
+    cols = grad.size(-1)
+    _check(h.shape == grad.shape and h.dtype in (grad.dtype, torch.float32),
+           "h must have grad's shape, and grad's dtype or float32")
+    _check(grad_h is None or (grad_h.shape == h.shape and grad_h.dtype == h.dtype),
+           "grad_h must have h's shape and dtype")
+    _check(rstd.device == dev and rstd.dtype == torch.float32 and rstd.is_contiguous()
+           and rstd.shape == grad.shape[:-1], "rstd must be the contiguous float32 tensor that rms_norm returned")
+    weight_type = dtype
+    if weight is not None:
+        _check(weight.device == dev and tuple(weight.shape) == (cols,) and weight.is_contiguous()
+               and weight.dtype in (grad.dtype, torch.float32),
+               "weight must be contiguous [columns of grad] on %s, of grad's dtype or float32" % dev)
+        weight_type = _ROW_TYPES[weight.dtype]
+    drop = _drop_args(dropout, dev)
+    grad_stride, h_stride = _row_stride(grad, "grad", dev), _row_stride(h, "h", dev)
+    gh_stride = 0 if grad_h is None else _row_stride(grad_h, "grad_h", dev)
+    grad_x = torch.empty(grad.shape, dtype=grad.dtype, device=dev)
+    apart = residual_grad and (dropout is not None or h.dtype != grad.dtype)
+    grad_res = torch.empty(grad.shape, dtype=h.dtype, device=dev) if apart else None
+    grad_w = ws = None
+    if weight is not None and weight_grad:
+        grad_w = torch.empty_like(weight)
+        ws = torch.empty(_lib.query("hades_rms_norm_grad_workspace_bytes", rstd.numel(), cols), dtype=torch.uint8,
+                         device=dev)
+    _lib.call("hades_rms_norm_grad", _ptr(grad), grad_stride, _ptr(h), h_stride, _opt(weight), _ptr(rstd),
+              _opt(grad_h), gh_stride, _ptr(grad_x), _opt(grad_res), _opt(grad_w), rstd.numel(), cols, dtype,
+              _ROW_TYPES[h.dtype], weight_type, *drop, _opt(ws), 0 if ws is None else ws.numel(), _stream())
+    return grad_x, (grad_res if apart else grad_x) if residual_grad else None, grad_w

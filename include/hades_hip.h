@@ -33,6 +33,9 @@ extern "C" {
 /* element type of row payloads (reference: FLOAT_TYPE_SWITCH, src/utils.h:26-37) */
 #define HADES_F32 0
 #define HADES_F64 1
+/* further element types of the input-stage operators (group 3) only */
+#define HADES_F16 2
+#define HADES_BF16 3
 /* index type (reference: INTEGER_TYPE_SWITCH, src/utils.h:39-50) */
 #define HADES_I32 0
 #define HADES_I64 1
@@ -55,7 +58,7 @@ extern "C" {
 const char* hades_last_error(void);
 /* Version of this interface; raised whenever a signature changes, so that a binding can refuse a
  * library built from other sources. */
-#define HADES_ABI_VERSION 131
+#define HADES_ABI_VERSION 132
 int hades_version(void);
 
 /* Kernel timing hook (no counterpart in the reference, whose scripts time whole calls from the
@@ -624,6 +627,61 @@ int hades_coldcache_flush(int64_t num_slots, int64_t dim, int32_t cnt_threshold,
                           int64_t lines, int64_t* out_ids, float* out_grads, int64_t* out_cnts,
                           int64_t* num_out, int64_t out_cap, void* workspace,
                           size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* Group 3: the input stage of a model over an embedding (no counterpart in the reference, whose
+ * rows leave the cache in float32 and go to the model as they are).  Element types: HADES_F32,
+ * HADES_F16, HADES_BF16; arithmetic in float32, one rounding where a value is stored.  Strides are
+ * in elements between rows whose values are contiguous; outputs without a stride are dense.
+ *
+ * Dropout is given by p, seed, offset and offset_ptr: threshold = round(p * 65536); value (row,
+ * column) is kept if 16 bits of Philox4x32 with 7 rounds - key = seed, counter = (column / 8, row,
+ * offset mod 2^32, offset / 2^32), bits = half column % 2 of word (column % 8) / 2 - reach it, and
+ * is then multiplied by 65536 / (65536 - threshold); else it is 0, whatever it was.  offset_ptr (device,
+ * may be NULL) is read when the kernel runs and added to offset.  p = 0 switches it off. */
+
+/* out[i, :] = dropout(scale * weight[ids[i], :]); an id outside [0, num_rows) gives a row of zeros */
+int hades_embed(const void* weight, int64_t weight_stride, int64_t num_rows, const void* ids, int64_t n,
+                void* out, int64_t dim, int dtype, int itype, float scale, double p, uint64_t seed,
+                int64_t offset, const int64_t* offset_ptr, void* stream);
+
+/* out[v, :] = sum over i with ids[i] = v of scale * dropout(grad[i, :]), every row of out written (zeros
+ * for tokens that do not occur); with accumulate != 0 the sum is added to out[v, :] and the rows of
+ * tokens that do not occur stay as they are.  Ids outside [0, num_rows) and padding_idx (negative: none)
+ * have no gradient.  out_dtype is dtype or HADES_F32.  Sums in float32, their order fixed by (n, dim) and
+ * the ids.  workspace: 256-byte aligned, needs no initialisation. */
+size_t hades_embed_grad_workspace_bytes(int64_t n, int64_t dim, int64_t num_rows);
+int hades_embed_grad(const void* grad, int64_t grad_stride, const void* ids, int64_t n, void* out,
+                     int64_t out_stride, int64_t num_rows, int64_t dim, int dtype, int out_dtype, int itype,
+                     int64_t padding_idx, int accumulate, float scale, double p, uint64_t seed, int64_t offset,
+                     const int64_t* offset_ptr, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out = dropout(x) (+ residual, unless NULL); the gradient of x is the same call on the gradient of out,
+ * without residual.  out may be x or residual where their rows are dense. */
+int hades_dropout(const void* x, int64_t x_stride, const void* residual, int64_t res_stride, void* out,
+                  int64_t rows, int64_t cols, int dtype, double p, uint64_t seed, int64_t offset,
+                  const int64_t* offset_ptr, void* stream);
+
+/* h = residual + dropout(x); rstd = 1 / sqrt(mean(h^2) + eps); y = h * rstd * weight.
+ * residual (type stream_dtype: dtype or HADES_F32), weight (weight_dtype: dtype or HADES_F32; NULL: ones), h
+ * (stream_dtype) and rstd may be NULL.  h may be residual where its rows are dense.  With scales != NULL, y
+ * is written as OCP e4m3 bytes in units of scales[rows][ceil(cols / group)], scale = max|y| / 448 over
+ * `group` columns (a power of two in [8, 512], or 0: the whole row); a group of zeros has scale 0, one with
+ * an infinity or a NaN a scale that is one too. */
+int hades_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t res_stride, const void* weight,
+                   void* y, float* scales, void* h, float* rstd, int64_t rows, int64_t cols, int dtype,
+                   int stream_dtype, int weight_dtype, int64_t group, float eps, double p, uint64_t seed,
+                   int64_t offset, const int64_t* offset_ptr, void* stream);
+
+/* With n = h * rstd and a = grad * weight: grad_res = rstd * (a - n * mean(a * n)) + grad_h (NULL: 0),
+ * grad_x = dropout(grad_res), grad_weight = sum over rows of grad * n.  grad_res (stream_dtype) and
+ * grad_weight (weight_dtype) may be NULL; workspace is for grad_weight, as for hades_embed_grad. */
+size_t hades_rms_norm_grad_workspace_bytes(int64_t rows, int64_t cols);
+int hades_rms_norm_grad(const void* grad, int64_t grad_stride, const void* h, int64_t h_stride, const void* weight,
+                        const float* rstd, const void* grad_h, int64_t grad_h_stride, void* grad_x, void* grad_res,
+                        void* grad_weight, int64_t rows, int64_t cols, int dtype, int stream_dtype,
+                        int weight_dtype, double p, uint64_t seed, int64_t offset, const int64_t* offset_ptr,
+                        void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
