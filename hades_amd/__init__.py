@@ -1,10 +1,13 @@
 """hades_amd - the HADES per-GPU embedding-cache hot path on MI355X (gfx950).
 
     hades_amd.EmbCacheLib   drop-in for the reference's extension module (same operator names)
-    hades_amd.ops           fused operators: lookup, split, cached_fetch/set, combine, optimizers
+    hades_amd.ops           fused operators: lookup, split, cached_fetch/set, combine, optimizers,
+                            embedding with scaling, dropout, RMS norm
     hades_amd.cache         EmbCache: hot-row cache keyed by the sorted hot-ID set
     hades_amd.sparse_optim  only_unique_grads / unique_grads / bucket_gradients / SparseAdagrad / SparseAdam
-    hades_amd.dist_emb      DistEmb / DistEmbeddingTensor and the trace-driven SparseAdam / SparseAdagrad
+    hades_amd.functional    embed / dropout / rms_norm with their gradients for torch.autograd
+    hades_amd.dist_emb      DistEmb / DistEmbeddingTensor and the trace-driven SparseAdam / SparseAdagrad;
+                            TokenEmb and InputStage
     hades_amd.index_cache   IndexCache / LocalCache: the set-associative index cache, in HBM
     hades_amd.cold_cache    ColdDataCache: the cache server's gradient path with its staleness rule
     hades_amd.shm           shared-memory segments and tensors, ShmTensorPool

@@ -15,11 +15,16 @@ or in its HBM, and the hot rows are the ids whose hotness reaches `hot_threshold
     rows = emb(ids)                  # lookup + hot/cold split + both gathers + sort of the keys
     loss(model(rows)).backward()
     opt.step()                       # segmented sums, mean over duplicate ids, fused row updates
+
+What a model does with its rows first - dropout, the addition to a residual stream, a root-mean-square
+norm, the rounding to 8 bits - is InputStage, which DistEmb (dropout=, norm=) and TokenEmb (a vocabulary
+table in HBM with a dense gradient) share.  None of it has a counterpart in the reference.
 """
 import torch
 import torch.nn as nn
 
 from . import cache as _cache
+from . import functional as _functional
 from . import ops
 from . import sparse_optim as _engine
 
@@ -118,14 +123,101 @@ class DistEmbeddingTensor:
         return self._fetch_only(ids.to(self._device).long())
 
 
+class InputStage(nn.Module):
+    """What rows go through on their way into a model: h = residual + dropout(rows), and with `norm`
+    y = h / sqrt(mean(h^2) + norm_eps) * weight.
+
+    The masks of a module are drawn from (seed, offset); without an explicit offset every forward call in
+    training takes the next one (kept with the state dict).  A captured forward needs `offset`, an int64
+    tensor of one element on the device that the captured step counts up itself: replays of one number
+    would drop the same values every time."""
+
+    def __init__(self, dim, dtype, dropout=0.0, norm=False, norm_eps=1e-6, seed=0, device="cuda"):
+        super().__init__()
+        if not 0.0 <= dropout <= 1.0:
+            raise RuntimeError("dropout must lie in [0, 1]")
+        self.dropout, self.norm_eps, self.seed = float(dropout), float(norm_eps), int(seed)
+        self.weight = nn.Parameter(torch.ones(dim, dtype=dtype, device=device)) if norm else None
+        self._calls = 0
+
+    def get_extra_state(self):
+        return {"calls": self._calls}
+
+    def set_extra_state(self, state):
+        self._calls = int(state["calls"])
+
+    def draw(self, offset=None):
+        """(p, seed, offset) of this forward call's mask, or None outside training."""
+        if not self.training or self.dropout == 0.0:
+            return None
+        if offset is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a captured forward with dropout needs an offset tensor on the device")
+            offset = self._calls
+            self._calls += 1
+        return self.dropout, self.seed, offset
+
+    def forward(self, rows, residual=None, offset=None):
+        """h, or with norm the pair (y, h)."""
+        drop = self.draw(offset)
+        if self.weight is not None:
+            return _functional.rms_norm(rows, self.weight, self.norm_eps, residual=residual, dropout=drop)
+        if drop is not None:
+            return _functional.dropout(rows, *drop, residual=residual)
+        return rows if residual is None else rows + residual
+
+    def forward_8bit(self, rows, residual=None, group=0):
+        """(q, scales, h) for an 8-bit product (ops.rms_norm_8bit): no dropout, no gradient."""
+        with torch.no_grad():
+            return ops.rms_norm_8bit(rows, self.weight, self.norm_eps, residual=residual, group=group)
+
+
+class TokenEmb(nn.Module):
+    """The embedding of a vocabulary that lives in HBM as a whole: rows of `dtype` (float32, float16,
+    bfloat16) times `scale`, then InputStage.  The counterpart of DistEmb for tables that a dense optimizer
+    updates: weight.grad is the dense gradient, summed by sorted tokens in float32 and the same from run
+    to run.  Ids outside [0, num_rows) are padding: rows of zeros without a gradient; the row of
+    `padding_idx` is used but gets no gradient."""
+
+    def __init__(self, num_rows, dim, dtype=torch.bfloat16, scale=1.0, padding_idx=None, dropout=0.0, norm=False,
+                 norm_eps=1e-6, seed=0, weight=None, device="cuda"):
+        super().__init__()
+        if weight is None:
+            weight = torch.empty((num_rows, dim), dtype=torch.float32).normal_(0.0, dim ** -0.5).to(dtype)
+        if tuple(weight.shape) != (num_rows, dim) or weight.dtype != dtype:
+            raise RuntimeError("weight must be [num_rows, dim] of dtype")
+        if padding_idx is not None and not 0 <= padding_idx < num_rows:
+            raise RuntimeError("padding_idx must be in [0, num_rows)")
+        self.weight = nn.Parameter(weight.to(device))
+        self.scale, self.padding_idx = float(scale), padding_idx
+        self.stage = InputStage(dim, dtype, dropout, norm, norm_eps, seed, device)
+
+    def forward(self, ids, residual=None, offset=None):
+        """Rows of ids.shape + (dim,) (with norm: the pair (y, h)), `residual` added if given."""
+        if self.stage.weight is None and residual is None:        # lookup and dropout in one kernel
+            return _functional.embed(self.weight, ids, self.scale, self.padding_idx, self.stage.draw(offset))
+        rows = _functional.embed(self.weight, ids, self.scale, self.padding_idx)
+        return self.stage(rows, residual, offset)
+
+    def forward_8bit(self, ids, residual=None, group=0):
+        """(q, scales, h) of the rows, as InputStage.forward_8bit."""
+        with torch.no_grad():
+            return self.stage.forward_8bit(ops.embed(self.weight, ids, scale=self.scale), residual, group)
+
+
 class DistEmb(nn.Module):
-    """python/EmbCache/dist_emb.py:11-52."""
+    """python/EmbCache/dist_emb.py:11-52.  Keyword-only additions to the reference's arguments: those of
+    DistEmbeddingTensor, and `dropout`, `norm`, `norm_eps`, `seed` of InputStage (without them the module
+    returns the rows as the reference does)."""
 
     def __init__(self, num_nodes, emb_dim, emb_dtype, name, cache_rate=0.3, idx_dtype=None,
                  local_rank=None, local_trainer_num=None, hotness_list=None, hot_threshold=150,
-                 part_book=None, cache_server_addr=None, cache_server_port=None, **kw):
+                 part_book=None, cache_server_addr=None, cache_server_port=None, *, dropout=0.0,
+                 norm=False, norm_eps=1e-6, seed=0, **kw):
         super().__init__()
         self.emb_dim = emb_dim
+        self.stage = InputStage(emb_dim, emb_dtype, dropout, norm, norm_eps, seed,
+                                kw.get("device", "cuda")) if dropout or norm else None
         self.sparse_emb = DistEmbeddingTensor(
             num_nodes, emb_dim, emb_dtype, name, cache_rate=cache_rate, idx_dtype=idx_dtype,
             local_rank=local_rank, local_trainer_num=local_trainer_num, hotness_list=hotness_list,
@@ -133,8 +225,20 @@ class DistEmb(nn.Module):
             cache_server_port=cache_server_port, **kw)
         self._device = torch.device(kw.get("device", "cuda"))
 
-    def forward(self, idx):
-        return self.sparse_emb(idx, self._device, self.training)
+    def forward(self, idx, residual=None, offset=None):
+        """The rows of idx; with dropout or norm, what InputStage makes of them and `residual`."""
+        rows = self.sparse_emb(idx, self._device, self.training)
+        if self.stage is None:
+            if residual is not None or offset is not None:
+                raise RuntimeError("residual and offset go with dropout or norm")
+            return rows
+        return self.stage(rows, residual, offset)
+
+    def forward_8bit(self, idx, residual=None, group=0):
+        """(q, scales, h) of the rows, normalised and in 8 bits (ops.rms_norm_8bit), without a trace."""
+        if self.stage is None or self.stage.weight is None:
+            raise RuntimeError("forward_8bit goes with norm")
+        return self.stage.forward_8bit(self.sparse_emb(idx, self._device, False), residual, group)
 
     def timecheck(self):
         pass
