@@ -21,39 +21,45 @@ constexpr int kThreads = 256;
 constexpr float kE4m3Max = 448.0f;
 constexpr int64_t kMaxPieces = 2048;   // of a row that stays in registers
 constexpr int64_t kMostThreads = int64_t(1) << 32;   // of a launch
+constexpr int64_t kCus = 256;
+// Pieces of a row up to which a lane of the gradient kernel holds one, else two: from 13 waves on only one
+// block of the one-piece form fits a compute unit, and nothing hides its waits for the row's sum (2^26
+// bfloat16 values with dropout in rows of 7 168 / 8 192: one piece 156 / 148 us, two 144 / 138).
+constexpr int64_t kGradOne = 768;
 
-__device__ __forceinline__ f32x8 load8_as(const void* p, int64_t at, bool f32, int valid, const float*) {
-  (void)f32;
-  return load8(static_cast<const float*>(p) + at, valid);
-}
-// a tensor whose type is the rows' T, or float32
+constexpr int kMaxWaves = 16;   // of a block
+
+// a weight, whose type is the rows' T or float32
 template <typename T>
-__device__ __forceinline__ f32x8 load8_as(const void* p, int64_t at, bool f32, int valid, const T*) {
-  return f32 ? load8(static_cast<const float*>(p) + at, valid) : load8(static_cast<const T*>(p) + at, valid);
-}
-template <typename T>
-__device__ __forceinline__ void store8_as(void* p, int64_t at, bool f32, f32x8 v, int valid, const T*) {
-  if (f32) store8(static_cast<float*>(p) + at, v, valid);
-  else store8(static_cast<T*>(p) + at, v, valid);
+__device__ __forceinline__ f32x8 load_weight(const void* p, int64_t piece, bool f32, int valid) {
+  return f32 ? load8(static_cast<const float*>(p) + piece * kPiece, valid)
+             : load8(static_cast<const T*>(p) + piece * kPiece, valid);
 }
 
-__device__ __forceinline__ float sum8(f32x8 v) {
-  return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+// a * b summed
+__device__ __forceinline__ float dot8(f32x8 a, f32x8 b) {
+  float lo = a[0] * b[0], hi = a[1] * b[1];
+#pragma unroll
+  for (int j = 2; j < kPiece; j += 2) {
+    lo = fmaf(a[j], b[j], lo);
+    hi = fmaf(a[j + 1], b[j + 1], hi);
+  }
+  return lo + hi;
 }
 
-// Sum over the T lanes of a row; every lane gets it.  For T > 64 `shared` has T / 64 values and all
-// threads of the block call (T is the block's size then).
+// Sum over the lanes of a row: T lanes of a wave, or (T = 0) the whole block, all of whose threads
+// call; `shared` has kMaxWaves values then.
 template <int T>
 __device__ __forceinline__ float row_sum(float v, float* shared) {
 #pragma unroll
-  for (int d = 1; d < (T < kWave ? T : kWave); d <<= 1) v += __shfl_xor(v, d, kWave);
-  if (T > kWave) {
+  for (int d = 1; d < (T ? T : kWave); d <<= 1) v += __shfl_xor(v, d, kWave);
+  if (T == 0) {
+    const int waves = blockDim.x / kWave;
     __syncthreads();   // `shared` may still be read for the value before
     if ((threadIdx.x & (kWave - 1)) == 0) shared[threadIdx.x / kWave] = v;
     __syncthreads();
     v = shared[0];
-#pragma unroll
-    for (int w = 1; w < T / kWave; ++w) v += shared[w];
+    for (int w = 1; w < waves; ++w) v += shared[w];
   }
   return v;
 }
@@ -68,26 +74,26 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v, int lanes) {
   return v;
 }
 
+// (a NaN among them is the largest here too)
 __device__ __forceinline__ uint32_t max8(f32x8 v) {
-  uint32_t m = 0;
+  float m = fabsf(v[0]);
 #pragma unroll
-  for (int j = 0; j < kPiece; ++j) {
-    const uint32_t b = __float_as_uint(v[j]) & 0x7fffffffu;
-    m = b > m ? b : m;
-  }
-  return m;
+  for (int j = 1; j < kPiece; ++j) m = __builtin_elementwise_maximum(m, fabsf(v[j]));
+  return __float_as_uint(m) & 0x7fffffffu;
 }
 
-// eight values in units of `scale`, rounded to e4m3 (nearest even); a group of zeros (scale 0) gives
-// zeros.  The division is the one of the definition: a product with 1 / scale could land on the other
-// side of a tie, and would overflow for the smallest scales.
+// Eight values in units of `scale`, rounded to e4m3 (nearest even).  scale is the largest magnitude of
+// the group over 448, so a value in its units is at most 448 (1 + 2^-22), which rounds to 448, the type's
+// largest.  One division a piece, its reciprocal times each value: a value next to a tie may fall to the
+// other side of it than the quotient would, 2^-23 of it away.  Where the reciprocal would overflow, or scale is
+// subnormal and coarse, every value is divided; a group of zeros (scale 0) gives zeros.
 __device__ __forceinline__ void store_e4m3(uint8_t* __restrict__ p, f32x8 v, float scale, int valid) {
-  float u[kPiece];
+  f32x8 u;
+  if (scale >= 0x1p-120f) {
+    u = v * (1.0f / scale);
+  } else {
 #pragma unroll
-  for (int j = 0; j < kPiece; ++j) {
-    const float r = scale > 0.0f ? v[j] / scale : 0.0f;
-    // (a NaN stays one: both comparisons are false)
-    u[j] = r > kE4m3Max ? kE4m3Max : (r < -kE4m3Max ? -kE4m3Max : r);
+    for (int j = 0; j < kPiece; ++j) u[j] = scale > 0.0f ? v[j] / scale : 0.0f;
   }
   int lo = 0, hi = 0;
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], lo, false);
@@ -116,7 +122,7 @@ struct NormArgs {
   float* rstd;            // may be null
   float* scales;
   int64_t x_stride, res_stride, rows, cols;
-  int stream_f32, weight_f32;
+  int weight_f32;
   int group_lanes;        // lanes that share a scale; 0: the row
   int64_t groups;         // scales of a row
   float eps;
@@ -128,42 +134,40 @@ __device__ __forceinline__ int valid_of(int64_t cols, int64_t piece) {
   return left <= 0 ? 0 : (left < kPiece ? static_cast<int>(left) : kPiece);
 }
 
-template <typename X>
+template <typename X, typename S>
 __device__ __forceinline__ f32x8 load_h(const NormArgs& a, const DropKeys& keys, int64_t row, int64_t piece, int valid) {
-  const X* tag = nullptr;
   f32x8 v = load8(static_cast<const X*>(a.x) + row * a.x_stride + piece * kPiece, valid);
   f32x8 r;
-  if (a.residual != nullptr)
-    r = load8_as(a.residual, row * a.res_stride + piece * kPiece, a.stream_f32, valid, tag);
+  if (a.residual != nullptr) r = load8(static_cast<const S*>(a.residual) + row * a.res_stride + piece * kPiece, valid);
   if (keys.on()) v = keys.apply(v, static_cast<uint32_t>(row), static_cast<uint32_t>(piece));
   if (a.residual != nullptr) v += r;
   return v;
 }
 
-template <typename X, int T, int K, bool kEight>
-__global__ __launch_bounds__(T > kThreads ? T : kThreads) void rms_norm_kernel(NormArgs a) {
-  constexpr int kRows = T > kThreads ? 1 : kThreads / T;
-  __shared__ float shared[T > kWave ? T / kWave : 1];
-  const X* tag = nullptr;
+// T lanes of a wave and K pieces of a row each, or T = 0: the lanes of a block
+template <typename X, typename S, int T, int K, bool kEight>
+__global__ __launch_bounds__(T ? kThreads : kMaxWaves* kWave) void rms_norm_kernel(NormArgs a) {
+  __shared__ float shared[kMaxWaves];
   const DropKeys keys(a.drop);
-  const int lane = threadIdx.x % T;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / T;
+  const int lanes = T ? T : blockDim.x;
+  const int lane = T ? threadIdx.x % T : threadIdx.x;
+  const int64_t row = T ? static_cast<int64_t>(blockIdx.x) * (kThreads / (T ? T : 1)) + threadIdx.x / (T ? T : 1)
+                        : static_cast<int64_t>(blockIdx.x);
   const bool in = row < a.rows;
   f32x8 h[K], w[K];
   int valid[K];
   float ss = 0.0f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int64_t piece = k * T + lane;
+    const int64_t piece = k * lanes + lane;
     valid[k] = in ? valid_of(a.cols, piece) : 0;
-    h[k] = load_h<X>(a, keys, row, piece, valid[k]);
-    if (a.weight != nullptr) w[k] = load8_as(a.weight, piece * kPiece, a.weight_f32, valid[k], tag);
+    h[k] = load_h<X, S>(a, keys, row, piece, valid[k]);
+    if (a.weight != nullptr) w[k] = load_weight<X>(a.weight, piece, a.weight_f32, valid[k]);
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    if (a.h != nullptr)
-      store8_as(a.h, row * a.cols + (k * T + lane) * kPiece, a.stream_f32, h[k], valid[k], tag);
-    ss += sum8(h[k] * h[k]);
+    if (a.h != nullptr) store8(static_cast<S*>(a.h) + row * a.cols + (k * lanes + lane) * kPiece, h[k], valid[k]);
+    ss += dot8(h[k], h[k]);
   }
   ss = row_sum<T>(ss, shared);
   const float rstd = 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps);
@@ -174,7 +178,7 @@ __global__ __launch_bounds__(T > kThreads ? T : kThreads) void rms_norm_kernel(N
     h[k] *= rstd;
     if (a.weight != nullptr) h[k] *= w[k];
     if (!kEight) {
-      store8(static_cast<X*>(a.y) + row * a.cols + (k * T + lane) * kPiece, h[k], valid[k]);
+      store8(static_cast<X*>(a.y) + row * a.cols + (k * lanes + lane) * kPiece, h[k], valid[k]);
     } else if (a.group_lanes == 0) {
       const uint32_t m = max8(h[k]);
       top = m > top ? m : top;
@@ -182,21 +186,20 @@ __global__ __launch_bounds__(T > kThreads ? T : kThreads) void rms_norm_kernel(N
   }
   if (!kEight) return;
   if (a.group_lanes == 0) {
-    __shared__ uint32_t tops[T > kWave ? T / kWave : 1];
-    top = lanes_max(top, T < kWave ? T : kWave);
-    if (T > kWave) {
+    __shared__ uint32_t tops[kMaxWaves];
+    top = lanes_max(top, T ? T : kWave);
+    if (T == 0) {
       if ((threadIdx.x & (kWave - 1)) == 0) tops[threadIdx.x / kWave] = top;
       __syncthreads();
       top = tops[0];
-#pragma unroll
-      for (int i = 1; i < T / kWave; ++i) top = tops[i] > top ? tops[i] : top;
+      for (int i = 1; i < lanes / kWave; ++i) top = tops[i] > top ? tops[i] : top;
     }
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int piece = k * T + lane;
+    const int piece = k * lanes + lane;
     uint32_t m = top;
-    if (a.group_lanes != 0) m = lanes_max(max8(h[k]), a.group_lanes < T ? a.group_lanes : T);
+    if (a.group_lanes != 0) m = lanes_max(max8(h[k]), T && a.group_lanes > T ? T : a.group_lanes);
     const float scale = __uint_as_float(m) / kE4m3Max;
     const bool first = a.group_lanes == 0 ? piece == 0 : (piece & (a.group_lanes - 1)) == 0;
     if (first && valid[k] > 0) a.scales[row * a.groups + (a.group_lanes == 0 ? 0 : piece / a.group_lanes)] = scale;
@@ -205,12 +208,11 @@ __global__ __launch_bounds__(T > kThreads ? T : kThreads) void rms_norm_kernel(N
 }
 
 // rows of more than kMaxPieces pieces: h is made again for each step
-template <typename X, bool kEight>
+template <typename X, typename S, bool kEight>
 __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs a) {
   constexpr int T = 1024;
-  __shared__ float shared[T / kWave];
-  __shared__ uint32_t tops[T / kWave];
-  const X* tag = nullptr;
+  __shared__ float shared[kMaxWaves];
+  __shared__ uint32_t tops[kMaxWaves];
   const DropKeys keys(a.drop);
   const int64_t row = blockIdx.x;
   const int64_t pieces = (a.cols + kPiece - 1) / kPiece;
@@ -218,11 +220,10 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs a) {
   float ss = 0.0f;
   for (int64_t k = 0; k < rounds; ++k) {
     const int64_t piece = k * T + threadIdx.x;
-    const int valid = valid_of(a.cols, piece);
-    const f32x8 h = load_h<X>(a, keys, row, piece, valid);
-    ss += sum8(h * h);
+    const f32x8 h = load_h<X, S>(a, keys, row, piece, valid_of(a.cols, piece));
+    ss += dot8(h, h);
   }
-  ss = row_sum<T>(ss, shared);
+  ss = row_sum<0>(ss, shared);
   const float rstd = 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps);
   if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = rstd;
   uint32_t top = 0;
@@ -230,24 +231,24 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs a) {
     for (int64_t k = 0; k < rounds; ++k) {
       const int64_t piece = k * T + threadIdx.x;
       const int valid = valid_of(a.cols, piece);
-      f32x8 y = load_h<X>(a, keys, row, piece, valid) * rstd;
-      if (a.weight != nullptr) y *= load8_as(a.weight, piece * kPiece, a.weight_f32, valid, tag);
+      f32x8 y = load_h<X, S>(a, keys, row, piece, valid) * rstd;
+      if (a.weight != nullptr) y *= load_weight<X>(a.weight, piece, a.weight_f32, valid);
       const uint32_t m = max8(y);
       top = m > top ? m : top;
     }
     top = lanes_max(top, kWave);
     if ((threadIdx.x & (kWave - 1)) == 0) tops[threadIdx.x / kWave] = top;
     __syncthreads();
-    for (int i = 0; i < T / kWave; ++i) top = tops[i] > top ? tops[i] : top;
+    for (int i = 0; i < kMaxWaves; ++i) top = tops[i] > top ? tops[i] : top;
   }
   for (int64_t k = 0; k < rounds; ++k) {
     const int64_t piece = k * T + threadIdx.x;
     const int valid = valid_of(a.cols, piece);
     const int64_t at = row * a.cols + piece * kPiece;
-    f32x8 y = load_h<X>(a, keys, row, piece, valid);
-    if (a.h != nullptr) store8_as(a.h, at, a.stream_f32, y, valid, tag);
+    f32x8 y = load_h<X, S>(a, keys, row, piece, valid);
+    if (a.h != nullptr) store8(static_cast<S*>(a.h) + at, y, valid);
     y *= rstd;
-    if (a.weight != nullptr) y *= load8_as(a.weight, piece * kPiece, a.weight_f32, valid, tag);
+    if (a.weight != nullptr) y *= load_weight<X>(a.weight, piece, a.weight_f32, valid);
     if (!kEight) {
       store8(static_cast<X*>(a.y) + at, y, valid);
       continue;
@@ -271,30 +272,29 @@ struct NormGradArgs {
   void* grad_res;        // may be null; the stream's type
   float* partial;        // [blocks][cols] rows of grad_weight's sum; null without grad_weight
   int64_t grad_stride, h_stride, grad_h_stride, rows, cols;
-  int stream_f32, weight_f32;
+  int weight_f32;
   DropArgs drop;
 };
 
 // A block takes every gridDim.x-th group of rows, so that a lane meets the same columns again and
-// keeps its part of grad_weight in registers until the end.
-template <typename X, int T, int K>
-__global__ __launch_bounds__(T > kThreads ? T : kThreads) void rms_norm_grad_kernel(NormGradArgs a) {
-  constexpr int kRows = T > kThreads ? 1 : kThreads / T;
-  __shared__ float shared[T > kWave ? T / kWave : 1];
-  __shared__ f32x8 parts[T < kThreads ? kThreads * K : 1];
-  const X* tag = nullptr;
+// keeps its part of grad_weight in registers until the end.  Lanes as in rms_norm_kernel.
+template <typename X, typename S, int T, int K>
+__global__ __launch_bounds__(T ? kThreads : kMaxWaves* kWave, T == 0 && K == 1 ? 6 : 1) void rms_norm_grad_kernel(NormGradArgs a) {
+  constexpr int kRows = T ? kThreads / (T ? T : 1) : 1;
+  __shared__ float shared[kMaxWaves];
+  __shared__ f32x8 parts[kRows > 1 ? kThreads * K : 1];
   const DropKeys keys(a.drop);
-  const int lane = threadIdx.x % T;
-  const int sub = threadIdx.x / T;
+  const int lanes = T ? T : blockDim.x;
+  const int lane = T ? threadIdx.x % T : threadIdx.x;
+  const int sub = T ? threadIdx.x / (T ? T : 1) : 0;
   const float inv_cols = 1.0f / static_cast<float>(a.cols);
   const f32x8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const f32x8 one = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
   f32x8 w[K], dw[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int64_t piece = k * T + lane;
+    const int64_t piece = k * lanes + lane;
     dw[k] = zero;
-    w[k] = a.weight != nullptr ? load8_as(a.weight, piece * kPiece, a.weight_f32, valid_of(a.cols, piece), tag) : one;
+    w[k] = a.weight != nullptr ? load_weight<X>(a.weight, piece, a.weight_f32, valid_of(a.cols, piece)) : zero + 1.0f;
   }
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.rows; base += static_cast<int64_t>(gridDim.x) * kRows) {
     const int64_t row = base + sub;
@@ -305,28 +305,27 @@ __global__ __launch_bounds__(T > kThreads ? T : kThreads) void rms_norm_grad_ker
     float dot = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int64_t piece = k * T + lane;
+      const int64_t piece = k * lanes + lane;
       valid[k] = in ? valid_of(a.cols, piece) : 0;
       g[k] = load8(static_cast<const X*>(a.grad) + row * a.grad_stride + piece * kPiece, valid[k]);
-      n[k] = load8_as(a.h, row * a.h_stride + piece * kPiece, a.stream_f32, valid[k], tag);
+      n[k] = load8(static_cast<const S*>(a.h) + row * a.h_stride + piece * kPiece, valid[k]);
       if (a.grad_h != nullptr)
-        gh[k] = load8_as(a.grad_h, row * a.grad_h_stride + piece * kPiece, a.stream_f32, valid[k], tag);
+        gh[k] = load8(static_cast<const S*>(a.grad_h) + row * a.grad_h_stride + piece * kPiece, valid[k]);
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       n[k] *= rstd;
-      dw[k] += g[k] * n[k];
+      dw[k] = __builtin_elementwise_fma(g[k], n[k], dw[k]);
       g[k] *= w[k];
-      dot += sum8(g[k] * n[k]);
+      dot += dot8(g[k], n[k]);
     }
     const float along = row_sum<T>(dot, shared) * inv_cols;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int64_t piece = k * T + lane;
+      const int64_t piece = k * lanes + lane;
       f32x8 d = (g[k] - n[k] * along) * rstd;
       if (a.grad_h != nullptr) d += gh[k];
-      if (a.grad_res != nullptr)
-        store8_as(a.grad_res, row * a.cols + piece * kPiece, a.stream_f32, d, valid[k], tag);
+      if (a.grad_res != nullptr) store8(static_cast<S*>(a.grad_res) + row * a.cols + piece * kPiece, d, valid[k]);
       if (keys.on()) d = keys.apply(d, static_cast<uint32_t>(row), static_cast<uint32_t>(piece));
       store8(static_cast<X*>(a.grad_x) + row * a.cols + piece * kPiece, d, valid[k]);
     }
@@ -343,17 +342,16 @@ __global__ __launch_bounds__(T > kThreads ? T : kThreads) void rms_norm_grad_ker
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int64_t piece = k * T + lane;
+    const int64_t piece = k * lanes + lane;
     store8(a.partial + blockIdx.x * a.cols + piece * kPiece, dw[k], valid_of(a.cols, piece));
   }
 }
 
 // rows of more than kMaxPieces pieces: the row is read again behind the sum
-template <typename X>
+template <typename X, typename S>
 __global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(NormGradArgs a) {
   constexpr int T = 1024;
-  __shared__ float shared[T / kWave];
-  const X* tag = nullptr;
+  __shared__ float shared[kMaxWaves];
   const DropKeys keys(a.drop);
   const int64_t row = blockIdx.x;
   const int64_t pieces = (a.cols + kPiece - 1) / kPiece;
@@ -362,34 +360,33 @@ __global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(NormGradArgs a
   for (int64_t piece = threadIdx.x; piece < pieces; piece += T) {
     const int valid = valid_of(a.cols, piece);
     f32x8 g = load8(static_cast<const X*>(a.grad) + row * a.grad_stride + piece * kPiece, valid);
-    if (a.weight != nullptr) g *= load8_as(a.weight, piece * kPiece, a.weight_f32, valid, tag);
-    dot += sum8(g * (load8_as(a.h, row * a.h_stride + piece * kPiece, a.stream_f32, valid, tag) * rstd));
+    if (a.weight != nullptr) g *= load_weight<X>(a.weight, piece, a.weight_f32, valid);
+    dot += dot8(g, load8(static_cast<const S*>(a.h) + row * a.h_stride + piece * kPiece, valid) * rstd);
   }
-  const float along = row_sum<T>(dot, shared) / static_cast<float>(a.cols);
+  const float along = row_sum<0>(dot, shared) / static_cast<float>(a.cols);
   for (int64_t piece = threadIdx.x; piece < pieces; piece += T) {
     const int valid = valid_of(a.cols, piece);
     f32x8 g = load8(static_cast<const X*>(a.grad) + row * a.grad_stride + piece * kPiece, valid);
-    if (a.weight != nullptr) g *= load8_as(a.weight, piece * kPiece, a.weight_f32, valid, tag);
-    const f32x8 n = load8_as(a.h, row * a.h_stride + piece * kPiece, a.stream_f32, valid, tag) * rstd;
+    if (a.weight != nullptr) g *= load_weight<X>(a.weight, piece, a.weight_f32, valid);
+    const f32x8 n = load8(static_cast<const S*>(a.h) + row * a.h_stride + piece * kPiece, valid) * rstd;
     f32x8 d = (g - n * along) * rstd;
-    if (a.grad_h != nullptr) d += load8_as(a.grad_h, row * a.grad_h_stride + piece * kPiece, a.stream_f32, valid, tag);
-    if (a.grad_res != nullptr) store8_as(a.grad_res, row * a.cols + piece * kPiece, a.stream_f32, d, valid, tag);
+    if (a.grad_h != nullptr) d += load8(static_cast<const S*>(a.grad_h) + row * a.grad_h_stride + piece * kPiece, valid);
+    if (a.grad_res != nullptr) store8(static_cast<S*>(a.grad_res) + row * a.cols + piece * kPiece, d, valid);
     if (keys.on()) d = keys.apply(d, static_cast<uint32_t>(row), static_cast<uint32_t>(piece));
     store8(static_cast<X*>(a.grad_x) + row * a.cols + piece * kPiece, d, valid);
   }
 }
 
 // ... and grad_weight's partial rows: block (x, y) takes kThreads pieces and every gridDim.y-th row
-template <typename X>
+template <typename X, typename S>
 __global__ __launch_bounds__(kThreads) void rms_norm_grad_weight_kernel(NormGradArgs a) {
-  const X* tag = nullptr;
   const int64_t piece = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const int valid = valid_of(a.cols, piece);
   if (valid == 0) return;
   f32x8 dw = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
     const f32x8 g = load8(static_cast<const X*>(a.grad) + row * a.grad_stride + piece * kPiece, valid);
-    dw += g * (load8_as(a.h, row * a.h_stride + piece * kPiece, a.stream_f32, valid, tag) * a.rstd[row]);
+    dw += g * (load8(static_cast<const S*>(a.h) + row * a.h_stride + piece * kPiece, valid) * a.rstd[row]);
   }
   store8(a.partial + blockIdx.y * a.cols + piece * kPiece, dw, valid);
 }
@@ -423,82 +420,75 @@ __global__ __launch_bounds__(kFoldWaves* kWave) void fold_rows_kernel(const floa
   out[col] = static_cast<W>(acc);
 }
 
-template <typename X, bool kEight>
+template <typename X, typename S, bool kEight>
 int launch_norm(const NormArgs& a, hipStream_t st) {
   const int64_t pieces = ceil_div(a.cols, kPiece);
-  if (pieces > kMaxPieces) {
-    HADES_REQUIRE(a.rows < kMostThreads / 1024, "rms_norm: too many rows for one call");
-    HADES_LAUNCH((rms_norm_long_kernel<X, kEight>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st, a);
-    return HADES_OK;
-  }
-#define HADES_NORM(T_, K_)                                                                              \
-  do {                                                                                                  \
-    constexpr int kBlock = T_ > kThreads ? T_ : kThreads;                                               \
-    const int64_t blocks = ceil_div(a.rows, kBlock / T_);                                               \
-    HADES_REQUIRE(blocks < kMostThreads / kBlock, "rms_norm: too many rows for one call");              \
-    HADES_LAUNCH((rms_norm_kernel<X, T_, K_, kEight>), dim3(static_cast<unsigned>(blocks)),             \
-                 dim3(kBlock), 0, st, a);                                                               \
-    return HADES_OK;                                                                                    \
+#define HADES_NORM(T_, K_)                                                                            \
+  do {                                                                                                \
+    const int64_t block = T_ ? kThreads : ceil_div(ceil_div(pieces, K_), kWave) * kWave;              \
+    const int64_t blocks = T_ ? ceil_div(a.rows, kThreads / (T_ ? T_ : 1)) : a.rows;                  \
+    HADES_REQUIRE(blocks < kMostThreads / block, "rms_norm: too many rows for one call");             \
+    HADES_LAUNCH((rms_norm_kernel<X, S, T_, K_, kEight>), dim3(static_cast<unsigned>(blocks)),        \
+                 dim3(static_cast<unsigned>(block)), 0, st, a);                                       \
+    return HADES_OK;                                                                                  \
   } while (0)
   if (pieces <= 8) HADES_NORM(8, 1);
   if (pieces <= 16) HADES_NORM(16, 1);
   if (pieces <= 32) HADES_NORM(32, 1);
   if (pieces <= 64) HADES_NORM(64, 1);
-  if (pieces <= 128) HADES_NORM(64, 2);
-  if (pieces <= 256) HADES_NORM(256, 1);
-  if (pieces <= 512) HADES_NORM(256, 2);
-  if (pieces <= 1024) HADES_NORM(256, 4);
-  HADES_NORM(512, 4);
+  if (pieces <= kMaxPieces / 2) HADES_NORM(0, 1);
+  if (pieces <= kMaxPieces) HADES_NORM(0, 2);
 #undef HADES_NORM
+  HADES_REQUIRE(a.rows < kMostThreads / 1024, "rms_norm: too many rows for one call");
+  HADES_LAUNCH((rms_norm_long_kernel<X, S, kEight>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st, a);
+  return HADES_OK;
 }
 
-// blocks of the gradient kernel: rows of grad_weight's partial sum
-constexpr int64_t kGradBlocks = 1024;
-
-int lanes_of(int64_t pieces) {
-  if (pieces > kMaxPieces) return 0;
-  if (pieces > 1024) return 512;
-  if (pieces > 128) return 256;
-  int t = 8;
-  while (t < kWave && t < pieces) t *= 2;
-  return t;
+// threads of a block of the gradient kernel
+int64_t grad_threads(int64_t pieces) {
+  if (pieces <= kWave) return kThreads;
+  return ceil_div(ceil_div(pieces, pieces <= kGradOne ? 1 : 2), kWave) * kWave;
 }
 
-int64_t grad_blocks(int64_t rows, int64_t cols) {
-  const int t = lanes_of(ceil_div(cols, kPiece));
-  const int64_t blocks = t == 0 ? rows : ceil_div(rows, t >= kThreads ? 1 : kThreads / t);
-  const int64_t most = t == 0 ? 64 : kGradBlocks;
-  return blocks < most ? blocks : most;
+// Blocks of the gradient kernel = rows of grad_weight's partial sum: as many as are resident at once, six
+// waves on each SIMD (80 registers) for 16-bit rows.  float32 rows have twice the bytes in flight: 16 waves a
+// compute unit do for them, and fewer partial rows are written (rows of 1 024: 139 us, with 24 waves 145).
+// The forms with 94 and 128 registers have five and four waves.
+int64_t grad_blocks(int64_t rows, int64_t cols, bool f32) {
+  const int64_t pieces = ceil_div(cols, kPiece);
+  if (pieces > kMaxPieces) return rows < 64 ? rows : 64;
+  int64_t lanes = 8;
+  while (lanes < kWave && lanes < pieces) lanes *= 2;
+  const int64_t blocks = pieces <= kWave ? ceil_div(rows, kThreads / lanes) : rows;
+  const int64_t waves = pieces <= kWave ? 20 : (pieces <= kGradOne && !f32 ? 24 : 16);
+  int64_t per_cu = waves / (grad_threads(pieces) / kWave);
+  if (per_cu < 1) per_cu = 1;
+  return blocks < per_cu * kCus ? blocks : per_cu * kCus;
 }
 
-template <typename X>
+template <typename X, typename S>
 int launch_norm_grad(const NormGradArgs& a, hipStream_t st) {
   const int64_t pieces = ceil_div(a.cols, kPiece);
-  const unsigned blocks = static_cast<unsigned>(grad_blocks(a.rows, a.cols));
-  if (pieces > kMaxPieces) {
-    HADES_REQUIRE(a.rows < kMostThreads / 1024, "rms_norm_grad: too many rows for one call");
-    HADES_LAUNCH((rms_norm_grad_long_kernel<X>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st, a);
-    if (a.partial != nullptr)
-      HADES_LAUNCH((rms_norm_grad_weight_kernel<X>), dim3(static_cast<unsigned>(ceil_div(pieces, kThreads)), blocks),
-                   dim3(kThreads), 0, st, a);
-    return HADES_OK;
-  }
-#define HADES_NORM_GRAD(T_, K_)                                                                          \
-  do {                                                                                                   \
-    HADES_LAUNCH((rms_norm_grad_kernel<X, T_, K_>), dim3(blocks), dim3(T_ > kThreads ? T_ : kThreads),   \
-                 0, st, a);                                                                              \
-    return HADES_OK;                                                                                     \
+  const unsigned blocks = static_cast<unsigned>(grad_blocks(a.rows, a.cols, sizeof(X) == 4));
+#define HADES_NORM_GRAD(T_, K_)                                                                        \
+  do {                                                                                                 \
+    HADES_LAUNCH((rms_norm_grad_kernel<X, S, T_, K_>), dim3(blocks),                                   \
+                 dim3(static_cast<unsigned>(grad_threads(pieces))), 0, st, a);                         \
+    return HADES_OK;                                                                                   \
   } while (0)
   if (pieces <= 8) HADES_NORM_GRAD(8, 1);
   if (pieces <= 16) HADES_NORM_GRAD(16, 1);
   if (pieces <= 32) HADES_NORM_GRAD(32, 1);
   if (pieces <= 64) HADES_NORM_GRAD(64, 1);
-  if (pieces <= 128) HADES_NORM_GRAD(64, 2);
-  if (pieces <= 256) HADES_NORM_GRAD(256, 1);
-  if (pieces <= 512) HADES_NORM_GRAD(256, 2);
-  if (pieces <= 1024) HADES_NORM_GRAD(256, 4);
-  HADES_NORM_GRAD(512, 4);
+  if (pieces <= kGradOne) HADES_NORM_GRAD(0, 1);
+  if (pieces <= kMaxPieces) HADES_NORM_GRAD(0, 2);
 #undef HADES_NORM_GRAD
+  HADES_REQUIRE(a.rows < kMostThreads / 1024, "rms_norm_grad: too many rows for one call");
+  HADES_LAUNCH((rms_norm_grad_long_kernel<X, S>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st, a);
+  if (a.partial != nullptr)
+    HADES_LAUNCH((rms_norm_grad_weight_kernel<X, S>),
+                 dim3(static_cast<unsigned>(ceil_div(pieces, kThreads)), blocks), dim3(kThreads), 0, st, a);
+  return HADES_OK;
 }
 
 bool row_type(int dtype) { return dtype == HADES_F32 || dtype == HADES_F16 || dtype == HADES_BF16; }
@@ -540,23 +530,27 @@ int hades_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_
   a.res_stride = res_stride;
   a.rows = rows;
   a.cols = cols;
-  a.stream_f32 = stream_dtype == HADES_F32;
   a.weight_f32 = weight_dtype == HADES_F32;
   a.group_lanes = static_cast<int>(group / kPiece);
   a.groups = group == 0 ? 1 : ceil_div(cols, group);
   a.eps = eps;
   a.drop = drop;
   hipStream_t st = static_cast<hipStream_t>(stream);
-#define HADES_NORM_TYPE(X_) return scales != nullptr ? launch_norm<X_, true>(a, st) : launch_norm<X_, false>(a, st)
-  if (dtype == HADES_F32) HADES_NORM_TYPE(float);
-  if (dtype == HADES_F16) HADES_NORM_TYPE(f16);
-  HADES_NORM_TYPE(bf16);
+#define HADES_NORM_TYPE(X_, S_) \
+  return scales != nullptr ? launch_norm<X_, S_, true>(a, st) : launch_norm<X_, S_, false>(a, st)
+  if (dtype == HADES_F32) HADES_NORM_TYPE(float, float);
+  if (dtype == HADES_F16) {
+    if (stream_dtype == HADES_F16) HADES_NORM_TYPE(f16, f16);
+    HADES_NORM_TYPE(f16, float);
+  }
+  if (stream_dtype == HADES_BF16) HADES_NORM_TYPE(bf16, bf16);
+  HADES_NORM_TYPE(bf16, float);
 #undef HADES_NORM_TYPE
 }
 
 size_t hades_rms_norm_grad_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows < 0 || cols < 1) return 0;
-  const size_t b = static_cast<size_t>(grad_blocks(rows > 0 ? rows : 1, cols)) * cols * sizeof(float);
+  const size_t b = static_cast<size_t>(grad_blocks(rows > 0 ? rows : 1, cols, false)) * cols * sizeof(float);
   return (b + 255) & ~size_t(255);
 }
 
@@ -597,16 +591,18 @@ int hades_rms_norm_grad(const void* grad, int64_t grad_stride, const void* h, in
   a.grad_h_stride = grad_h_stride;
   a.rows = rows;
   a.cols = cols;
-  a.stream_f32 = stream_dtype == HADES_F32;
   a.weight_f32 = weight_dtype == HADES_F32;
   a.drop = drop;
   hipStream_t st = static_cast<hipStream_t>(stream);
   int rc = HADES_OK;
-  if (rows > 0)
-    rc = dtype == HADES_F32 ? launch_norm_grad<float>(a, st)
-                            : (dtype == HADES_F16 ? launch_norm_grad<f16>(a, st) : launch_norm_grad<bf16>(a, st));
+  if (rows > 0) {
+    if (dtype == HADES_F32) rc = launch_norm_grad<float, float>(a, st);
+    else if (dtype == HADES_F16)
+      rc = stream_dtype == HADES_F16 ? launch_norm_grad<f16, f16>(a, st) : launch_norm_grad<f16, float>(a, st);
+    else rc = stream_dtype == HADES_BF16 ? launch_norm_grad<bf16, bf16>(a, st) : launch_norm_grad<bf16, float>(a, st);
+  }
   if (rc != HADES_OK || !grad_weight) return rc;
-  const int64_t blocks = rows > 0 ? grad_blocks(rows, cols) : 0;
+  const int64_t blocks = rows > 0 ? grad_blocks(rows, cols, dtype == HADES_F32) : 0;
   const dim3 grid(static_cast<unsigned>(ceil_div(cols, kWave))), block(kFoldWaves * kWave);
 #define HADES_FOLD(W_) \
   HADES_LAUNCH((fold_rows_kernel<W_>), grid, block, 0, st, a.partial, blocks, cols, static_cast<W_*>(grad_weight))
