@@ -13,12 +13,15 @@
 // Gradient: every row of the dense gradient is written once, n rows of g are read once; sums are
 // held in float32 and their order is fixed by (n, dim) and the sorted tokens, so results are the same
 // from run to run.  Three parts:
-//   tokens  positions in token order (stable) and row_start[v] = first of token v
-//   sum     chunks of kShort or kLong sorted positions, whatever the tokens' frequencies: one lane
-//           group walks a chunk's rows for its columns and writes every token that lies inside the
-//           chunk; what crosses a border goes to a partial row.  Further blocks of the same launch
-//           write the zeros of the tokens that do not occur.
-//   join    adds the partial rows of the tokens that cross chunk borders, in chunk order.
+//   tokens  positions in token order (stable) and row_start[v] = first of token v: one kernel whose
+//           blocks each look through all ids for the tokens of their own range, or, for long batches
+//           and large tables, the library's radix sort
+//   sum     chunks of 8, 16 or 32 sorted positions, whatever the tokens' frequencies: one lane
+//           group walks the rows of a chunk for its columns and writes every token that begins in the
+//           chunk and ends there or in the next one, whose first rows it then takes too.  A longer
+//           token leaves a partial row in every chunk that it touches.  Further blocks of the same
+//           launch write the zeros of the tokens that do not occur.
+//   join    adds the partial rows of the long tokens, in chunk order.
 #include "internal.h"
 #include "rowvec.h"
 
@@ -26,10 +29,13 @@ namespace hades {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPieces = 4;    // pieces per thread of the flat kernels
-constexpr uint32_t kNoToken = 0xffffffffu;
+constexpr int kZeroUnits = 2;   // 16-byte units a thread zeroes (1.07 GB: 164 us; 1 or 4 units 203)
 
 // ---- lookup -------------------------------------------------------------------------------------
+// pieces of a thread: two 16-byte loads, whatever the type
+template <typename T>
+constexpr int embed_pieces() { return sizeof(T) == 2 ? 2 : 1; }
+
 template <typename T, typename I>
 struct EmbedArgs {
   const T* weight;
@@ -42,6 +48,7 @@ struct EmbedArgs {
 
 template <typename T, typename I>
 __global__ __launch_bounds__(kThreads) void embed_kernel(EmbedArgs<T, I> a) {
+  constexpr int kPieces = embed_pieces<T>();
   const DropKeys keys(a.drop);
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (kThreads * kPieces);
   const int64_t row0 = a.pieces < (int64_t(1) << 31) ? int64_t(a.per_row.div(uint32_t(first))) : first / a.per_row.d;
@@ -70,7 +77,7 @@ __global__ __launch_bounds__(kThreads) void embed_kernel(EmbedArgs<T, I> a) {
 #pragma unroll
   for (int k = 0; k < kPieces; ++k) {
     const f32x8 y = keys.on() ? keys.apply(v[k], static_cast<uint32_t>(row[k]), piece[k]) : v[k] * keys.factor;
-    store8(a.out + row[k] * a.dim + static_cast<int64_t>(piece[k]) * kPiece, y, valid[k]);
+    store8<T, true>(a.out + row[k] * a.dim + static_cast<int64_t>(piece[k]) * kPiece, y, valid[k]);
   }
 }
 
@@ -88,7 +95,7 @@ int launch_embed(const void* weight, int64_t stride, int64_t num_rows, const voi
   a.pieces = n * per_row;
   a.per_row = FastDiv(static_cast<uint32_t>(per_row));
   a.drop = drop;
-  const int64_t blocks = ceil_div(a.pieces, int64_t(kThreads) * kPieces);
+  const int64_t blocks = ceil_div(a.pieces, int64_t(kThreads) * embed_pieces<T>());
   HADES_REQUIRE(blocks < (int64_t(1) << 24), "embed: too many values for one call");
   HADES_LAUNCH((embed_kernel<T, I>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, a);
   return HADES_OK;
@@ -106,6 +113,152 @@ __global__ __launch_bounds__(kThreads) void token_key_kernel(const I* __restrict
   keys[i] = live ? id : num_rows;   // padding sorts behind every token
 }
 
+// Two kernels sort a batch of up to kTiles tiles: the first groups every tile's positions by bucket (a range
+// of 2^shift tokens), the second gives every bucket a block that fetches its pieces of all tiles and puts them
+// in token order.  Neither needs another block's result of the same launch, so the sort is two short launches
+// where the radix sort makes six to nine that wait for one another.
+constexpr int kTileIds = 1024;      // ids of a tile, a thread each
+constexpr int kTileWaves = kTileIds / kWave;
+constexpr int kTiles = 128;
+constexpr int kMinBucketBits = 8;   // a block for every compute unit
+constexpr int kMaxBucketBits = 10;
+constexpr int kMaxShift = 10;
+
+// lanes of the wave whose value agrees with the lane's in the low `bits` bits, among `of`
+__device__ __forceinline__ uint64_t peers_of(uint32_t v, int bits, uint64_t of) {
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (v >> b) & 1u;
+    const uint64_t ones = __ballot(one);
+    of &= one ? ones : ~ones;
+  }
+  return of;
+}
+
+// tok / pos [tile][kTileIds]: the tile's tokens and their positions, grouped by bucket in order of position;
+// offsets[bucket][tile]: where a bucket begins in its tile, [buckets][tile]: the tile's number of tokens
+template <typename I>
+__global__ __launch_bounds__(kTileIds) void token_tile_kernel(const I* __restrict__ ids, int64_t n, int64_t num_rows,
+                                                              int64_t padding, int shift, int bits, int tiles,
+                                                              uint32_t* __restrict__ tok, uint32_t* __restrict__ pos,
+                                                              uint32_t* __restrict__ offsets) {
+  extern __shared__ uint32_t counts[];   // [kTileWaves][2^bits]
+  __shared__ uint32_t scan[kTileWaves + 1];
+  const int buckets = 1 << bits;
+  const int wave = threadIdx.x / kWave;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kTileIds + threadIdx.x;
+  const int64_t id = i < n ? static_cast<int64_t>(ids[i]) : int64_t(-1);
+  const bool real = static_cast<uint64_t>(id) < static_cast<uint64_t>(num_rows) && id != padding;
+  const uint32_t bucket = real ? static_cast<uint32_t>(id) >> shift : 0u;
+  for (int k = threadIdx.x; k < kTileWaves * buckets; k += kTileIds) counts[k] = 0;
+  __syncthreads();
+  const uint64_t peers = peers_of(bucket, bits, __ballot(real));
+  const uint32_t rank = ballot_rank(peers);
+  if (real && rank == 0) counts[wave * buckets + bucket] = static_cast<uint32_t>(__popcll(peers));
+  __syncthreads();
+  uint32_t total = 0;
+  if (threadIdx.x < static_cast<uint32_t>(buckets)) {
+    for (int w = 0; w < kTileWaves; ++w) {
+      const uint32_t c = counts[w * buckets + threadIdx.x];
+      counts[w * buckets + threadIdx.x] = total;
+      total += c;
+    }
+  }
+  uint32_t all;
+  const uint32_t start = block_exclusive_sum<uint32_t, kTileIds>(total, scan, &all);
+  if (threadIdx.x < static_cast<uint32_t>(buckets)) {
+    offsets[static_cast<int64_t>(threadIdx.x) * tiles + blockIdx.x] = start;
+    for (int w = 0; w < kTileWaves; ++w) counts[w * buckets + threadIdx.x] += start;
+  }
+  if (threadIdx.x == 0) offsets[static_cast<int64_t>(buckets) * tiles + blockIdx.x] = all;
+  __syncthreads();
+  if (real) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kTileIds + counts[wave * buckets + bucket] + rank;
+    tok[at] = static_cast<uint32_t>(id);
+    pos[at] = static_cast<uint32_t>(i);
+  }
+}
+
+__global__ __launch_bounds__(kTileIds) void token_bucket_kernel(const uint32_t* __restrict__ tok,
+                                                                const uint32_t* __restrict__ pos,
+                                                                const uint32_t* __restrict__ offsets, int tiles,
+                                                                int64_t num_rows, int shift,
+                                                                uint32_t* __restrict__ perm,
+                                                                uint32_t* __restrict__ token,
+                                                                uint32_t* __restrict__ row_start) {
+  extern __shared__ uint32_t counts[];   // [kTileWaves][2^shift]
+  __shared__ uint32_t scan[kTileWaves + 1];
+  __shared__ uint32_t first[kTiles];     // of the bucket's list, in order of position: a tile's first entry
+  __shared__ uint32_t place[kTiles];     // entry e of tile t is tok[place[t] + e]
+  const int range = 1 << shift;
+  const uint32_t v0 = blockIdx.x << shift;
+  const uint32_t rows = static_cast<uint32_t>(num_rows);
+  const uint32_t mine = rows - v0 < static_cast<uint32_t>(range) ? rows - v0 : static_cast<uint32_t>(range);
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = threadIdx.x / kWave;
+  uint32_t begin = 0, size = 0;
+  if (static_cast<int>(threadIdx.x) < tiles) {
+    begin = offsets[static_cast<int64_t>(blockIdx.x) * tiles + threadIdx.x];
+    size = offsets[static_cast<int64_t>(blockIdx.x + 1) * tiles + threadIdx.x] - begin;
+  }
+  for (int k = threadIdx.x; k < kTileWaves * range; k += kTileIds) counts[k] = 0;
+  uint32_t list, base;   // length of the bucket's list, and tokens of the buckets below
+  const uint32_t entry = block_exclusive_sum<uint32_t, kTileIds>(size, scan, &list);
+  block_exclusive_sum<uint32_t, kTileIds>(begin, scan, &base);
+  if (static_cast<int>(threadIdx.x) < tiles) {
+    first[threadIdx.x] = entry;
+    place[threadIdx.x] = threadIdx.x * kTileIds + begin - entry;
+  }
+  __syncthreads();
+  // a wave takes a stretch of the list, so that places by wave, step and lane keep the order of positions
+  volatile uint32_t* const own = counts + wave * range;   // lanes read what other lanes of the wave wrote
+  const uint32_t part = (list + kTileIds - 1) / kTileIds * kWave;
+  const uint32_t lo = wave * part, hi = lo + part < list ? lo + part : list;
+  const auto where = [&](uint32_t e) {   // in tok and pos: the last tile whose first entry is not above e
+    int a = 0, b = tiles;
+    while (b - a > 1) {
+      const int mid = (a + b) >> 1;
+      if (first[mid] <= e) a = mid; else b = mid;
+    }
+    return place[a] + e;
+  };
+  for (uint32_t e = lo + lane; e - lane < hi; e += kWave) {
+    const bool in = e < hi;
+    const uint32_t at = in ? tok[where(e)] - v0 : 0u;
+    const uint64_t peers = peers_of(at, shift, __ballot(in));
+    if (in && ballot_rank(peers) == 0) own[at] = own[at] + static_cast<uint32_t>(__popcll(peers));
+  }
+  __syncthreads();
+  // a thread a token: the waves' counts become their first places
+  uint32_t total = 0;
+  if (threadIdx.x < mine) {
+    for (int w = 0; w < kTileWaves; ++w) {
+      const uint32_t c = counts[w * range + threadIdx.x];
+      counts[w * range + threadIdx.x] = total;
+      total += c;
+    }
+  }
+  const uint32_t start = base + block_exclusive_sum<uint32_t, kTileIds>(total, scan, &total);
+  if (threadIdx.x < mine) {
+    row_start[v0 + threadIdx.x] = start;
+    for (int w = 0; w < kTileWaves; ++w) counts[w * range + threadIdx.x] += start;
+  }
+  if (v0 + mine == rows && threadIdx.x == 0) row_start[rows] = base + list;
+  __syncthreads();
+  for (uint32_t e = lo + lane; e - lane < hi; e += kWave) {
+    const bool in = e < hi;
+    const uint32_t from = in ? where(e) : 0u;
+    const uint32_t at = in ? tok[from] - v0 : 0u;
+    const uint64_t peers = peers_of(at, shift, __ballot(in));
+    const uint32_t rank = ballot_rank(peers);
+    if (in) {
+      const uint32_t to = own[at];
+      perm[to + rank] = pos[from];
+      token[to + rank] = v0 + at;
+      if (rank == 0) own[at] = to + static_cast<uint32_t>(__popcll(peers));
+    }
+  }
+}
+
 // row_start[v] = number of sorted tokens below v, for v in [0, num_rows]
 __global__ __launch_bounds__(kThreads) void row_start_kernel(const uint32_t* __restrict__ token, int64_t n,
                                                              int64_t num_rows, uint32_t* __restrict__ row_start) {
@@ -120,9 +273,14 @@ __global__ __launch_bounds__(kThreads) void row_start_kernel(const uint32_t* __r
 }
 
 // ---- gradient: sums -----------------------------------------------------------------------------
-constexpr int kLong = 32;    // sorted positions of a chunk
-constexpr int kShort = 8;    // ... where chunks of kLong would leave the chip short of waves
-constexpr int64_t kLongFrom = 2048;   // waves
+// Sorted positions of a chunk: the fewer, the more waves and the more partial rows.  us of the whole
+// gradient with chunks of 8 / 16 / 32: 16 384 rows of 1 024 bfloat16 into 32 000: 44 / 39 / -, 65 536 rows of 999
+// float32: 150 / 135 / 144, 32 768 rows of 4 096 bfloat16 into 131 072: - / 244 / 237.
+constexpr int kChunkShort = 8;
+constexpr int kChunk = 16;
+constexpr int kChunkLong = 32;
+constexpr int64_t kChunkWaves = 2048;       // waves that chunks of kChunk have to give
+constexpr int64_t kChunkLongWaves = 8192;   // ... and of kChunkLong
 
 struct GradPlan {
   int group;        // lanes that walk a chunk's rows together: 8, 16, 32 or 64
@@ -138,8 +296,8 @@ GradPlan plan_grad(int64_t n, int64_t dim) {
   p.group = 8;
   while (p.group < kWave && p.group < p.pieces) p.group *= 2;
   p.slices = static_cast<int>(ceil_div(p.pieces, p.group));
-  const int64_t waves = ceil_div(ceil_div(n, kLong) * p.slices * p.group, kWave);
-  p.chunk = waves >= kLongFrom ? kLong : kShort;
+  const auto waves = [&](int chunk) { return ceil_div(ceil_div(n, chunk) * p.slices * p.group, kWave); };
+  p.chunk = waves(kChunkLong) >= kChunkLongWaves ? kChunkLong : (waves(kChunk) >= kChunkWaves ? kChunk : kChunkShort);
   p.chunks = ceil_div(n, p.chunk);
   return p;
 }
@@ -151,12 +309,13 @@ struct GradArgs {
   const uint32_t* token;       // its token
   const uint32_t* row_start;   // [num_rows + 1]
   O* out;
-  float* partial;              // [2 * chunks][dim]: of every chunk the token it begins inside, the one it ends inside
+  float* partial;              // [2 * chunks][dim], see is_long
   int64_t grad_stride, out_stride, num_rows, dim, chunks;
   int slices, accumulate;
+  int once;                    // rows of grad: see streamed
   unsigned sum_blocks;
   FastDiv per_row, per_chunk;
-  int64_t zero_pieces;
+  int64_t zero_units;
   DropArgs drop;
 };
 
@@ -167,26 +326,40 @@ __device__ __forceinline__ void put_row(const GradArgs<T, O>& a, uint32_t token,
   store8(p, v, valid);
 }
 
-__device__ __forceinline__ void put_partial(float* __restrict__ p, f32x8 v, int valid) { store8(p, v, valid); }
+// a token whose rows reach beyond the chunk behind the one that it begins in
+template <int CH>
+__device__ __forceinline__ bool is_long(int64_t begin, int64_t end) { return end > (begin / CH + 2) * CH; }
 
 template <typename T, typename O, int G, int CH>
 __global__ __launch_bounds__(kThreads) void embed_grad_sum_kernel(GradArgs<T, O> a) {
   if (blockIdx.x >= a.sum_blocks) {
-    // the rows of tokens that do not occur
-    const int64_t first = static_cast<int64_t>(blockIdx.x - a.sum_blocks) * (kThreads * kPieces);
-    const int64_t row0 = a.zero_pieces < (int64_t(1) << 31) ? int64_t(a.per_row.div(uint32_t(first)))
-                                                            : first / a.per_row.d;
+    // the rows of tokens that do not occur, in units of 16 bytes that are aligned whatever the rows are: the
+    // first and the last unit of a row may be part of one
+    constexpr int kUnit = 16 / sizeof(O);
+    typedef O UnitV __attribute__((ext_vector_type(kUnit)));
+    const int64_t first = static_cast<int64_t>(blockIdx.x - a.sum_blocks) * (kThreads * kZeroUnits);
+    const int64_t row0 = a.zero_units < (int64_t(1) << 31) ? int64_t(a.per_row.div(uint32_t(first)))
+                                                           : first / a.per_row.d;
     const uint32_t rest = static_cast<uint32_t>(first - row0 * a.per_row.d);
-    const f32x8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < kPieces; ++k) {
-      if (first + threadIdx.x + k * kThreads >= a.zero_pieces) break;
+    for (int k = 0; k < kZeroUnits; ++k) {
+      if (first + threadIdx.x + k * kThreads >= a.zero_units) break;
       const uint32_t at = rest + threadIdx.x + k * kThreads;
       const uint32_t down = a.per_row.div(at);
       const int64_t v = row0 + down;
       if (a.row_start[v] != a.row_start[v + 1]) continue;
-      const int64_t col = static_cast<int64_t>(at - down * a.per_row.d) * kPiece;
-      store8(a.out + v * a.out_stride + col, zero, a.dim - col < kPiece ? int(a.dim - col) : kPiece);
+      O* const row = a.out + v * a.out_stride;
+      const int64_t skew = static_cast<int64_t>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(O));
+      const int64_t col = static_cast<int64_t>(at - down * a.per_row.d) * kUnit - skew;
+      if (col >= 0 && a.dim - col >= kUnit) {
+        UnitV zero;
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) zero[j] = static_cast<O>(0.0f);
+        __builtin_nontemporal_store(zero, reinterpret_cast<UnitV*>(row + col));
+      } else {
+        for (int j = 0; j < kUnit; ++j)
+          if (col + j >= 0 && col + j < a.dim) row[col + j] = static_cast<O>(0.0f);
+      }
     }
     return;
   }
@@ -201,18 +374,30 @@ __global__ __launch_bounds__(kThreads) void embed_grad_sum_kernel(GradArgs<T, O>
   const int64_t left = a.dim - col;
   const int valid = left < 0 ? 0 : (left < kPiece ? static_cast<int>(left) : kPiece);
   const int64_t live = a.row_start[a.num_rows];
-  const int64_t p0 = static_cast<int64_t>(chunk) * CH;
+  int64_t p0 = static_cast<int64_t>(chunk) * CH;
   if (p0 >= live || valid == 0) return;
-  const int len = live - p0 < CH ? static_cast<int>(live - p0) : CH;
-  const uint32_t before = p0 > 0 ? a.token[p0 - 1] : kNoToken;
-  const uint32_t after = p0 + len < live ? a.token[p0 + len] : kNoToken;
+  int64_t p1 = p0 + CH < live ? p0 + CH : live;
+  // the chunk's first token began before it: the chunk before takes all of it, or it is a long one
   uint32_t cur = a.token[p0];
-  bool head = before == cur;   // the token summed now began in an earlier chunk
+  bool part = false;   // the token summed now is a long one: its row is partial
+  {
+    const int64_t begin = a.row_start[cur], end = a.row_start[cur + 1];
+    if (is_long<CH>(begin, end)) part = true;
+    else if (begin < p0) p0 = end;
+  }
+  // ... and the last one goes on behind it: taken to its end, unless it is long
+  const uint32_t last = a.token[p1 - 1];
+  const int64_t last_begin = a.row_start[last], last_end = a.row_start[last + 1];
+  if (last_begin >= static_cast<int64_t>(chunk) * CH && !is_long<CH>(last_begin, last_end)) p1 = last_end;
+  if (p0 >= p1) return;
+  cur = a.token[p0];
   const f32x8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   f32x8 acc = zero;
+  // slot 0: a long token that began earlier; slot 1: one that begins here
   float* const slot = a.partial + 2 * static_cast<int64_t>(chunk) * a.dim + col;
+  const int len = static_cast<int>(p1 - p0);
   for (int t = 0; t < len; t += U) {
-    f32x8 row[U];
+    typename Vec8<T>::V row[U];
     uint32_t tok[U], pos[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
@@ -220,70 +405,135 @@ __global__ __launch_bounds__(kThreads) void embed_grad_sum_kernel(GradArgs<T, O>
       pos[k] = a.perm[j];
       tok[k] = a.token[j];
     }
+    if (a.once) {
 #pragma unroll
-    for (int k = 0; k < U; ++k)
-      row[k] = load8<T, true>(a.grad + static_cast<int64_t>(pos[k]) * a.grad_stride + col, valid);
+      for (int k = 0; k < U; ++k)
+        row[k] = load8_raw<T, true>(a.grad + static_cast<int64_t>(pos[k]) * a.grad_stride + col, valid);
+    } else {
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        row[k] = load8_raw<T>(a.grad + static_cast<int64_t>(pos[k]) * a.grad_stride + col, valid);
+    }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       if (t + k >= len) break;
       if (tok[k] != cur) {
-        if (head) put_partial(slot, acc, valid);
+        if (part) store8(slot, acc, valid);   // (only the chunk's first token can end here as a long one)
         else put_row(a, cur, col, acc, valid);
         acc = zero;
         cur = tok[k];
-        head = false;
+        part = false;
       }
-      acc += keys.on() ? keys.apply(row[k], pos[k], piece) : row[k] * keys.factor;
+      const f32x8 v = __builtin_convertvector(row[k], f32x8);
+      acc += keys.on() ? keys.apply(v, pos[k], piece) : v * keys.factor;
     }
   }
-  if (head) put_partial(slot, acc, valid);
-  else if (after == cur) put_partial(slot + a.dim, acc, valid);
-  else put_row(a, cur, col, acc, valid);
+  if (part || (cur == last && is_long<CH>(last_begin, last_end))) {
+    const bool begins = static_cast<int64_t>(a.row_start[cur]) >= static_cast<int64_t>(chunk) * CH;
+    store8(slot + (begins ? a.dim : 0), acc, valid);
+  } else {
+    put_row(a, cur, col, acc, valid);
+  }
 }
 
-// Block (chunk c, slice): the token that begins in chunk c and goes on behind it, if there is one.
-// Its lane groups take the partial rows in turn; the groups' sums are added in order.
+// A block looks at kJoinChunks chunks for long tokens that begin in them, one a lane group at a time, and
+// adds their partial rows for one slice of columns.  A token of more than kJoinAlone parts is left to the
+// whole block: its groups take the parts in turn, and their sums are added in order.
+constexpr int kJoinThreads = 512;
+constexpr int kJoinChunks = 8;    // at most kJoinThreads / 64
+constexpr int kJoinAlone = 32;
+
 template <typename T, typename O, int G, int CH>
-__global__ __launch_bounds__(kThreads) void embed_grad_join_kernel(GradArgs<T, O> a) {
-  constexpr int kGroups = kThreads / G;
+__global__ __launch_bounds__(kJoinThreads) void embed_grad_join_kernel(GradArgs<T, O> a) {
+  constexpr int kGroups = kJoinThreads / G;
   constexpr int U = 8;
-  __shared__ f32x8 part[kThreads];
+  __shared__ f32x8 sums[kJoinThreads];
+  __shared__ uint32_t token_of[kJoinChunks];
+  __shared__ int parts_of[kJoinChunks];   // 0: no long token begins in the chunk
   const int64_t live = a.row_start[a.num_rows];
-  const int64_t c = a.per_chunk.div(blockIdx.x);
-  const int64_t border = (c + 1) * CH;
-  if (border >= live) return;
-  const uint32_t token = a.token[border - 1];
-  if (a.token[border] != token || static_cast<int64_t>(a.row_start[token]) < c * CH) return;
-  const int64_t parts = (static_cast<int64_t>(a.row_start[token + 1]) - 1) / CH - c + 1;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kJoinChunks;
+  if (threadIdx.x < kJoinChunks) {
+    const int64_t c = c0 + threadIdx.x, border = (c + 1) * CH;
+    int parts = 0;
+    if (border < live) {
+      const uint32_t token = a.token[border - 1];
+      const int64_t begin = a.row_start[token], end = a.row_start[token + 1];
+      if (begin >= c * CH && is_long<CH>(begin, end)) parts = static_cast<int>((end - 1) / CH - c + 1);
+      token_of[threadIdx.x] = token;
+    }
+    parts_of[threadIdx.x] = parts;
+  }
+  __syncthreads();
   const int group = threadIdx.x / G, lane = threadIdx.x & (G - 1);
-  const int64_t col = (static_cast<int64_t>(blockIdx.x - static_cast<uint32_t>(c) * a.slices) * G + lane) * kPiece;
+  const int64_t col = (static_cast<int64_t>(blockIdx.y) * G + lane) * kPiece;
   const int64_t left = a.dim - col;
   const int valid = left < 0 ? 0 : (left < kPiece ? static_cast<int>(left) : kPiece);
-  f32x8 acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int64_t t = group; t < parts; t += kGroups * U) {
-    f32x8 row[U];
+  // parts at, at + step, ... of the token that begins in chunk c
+  const auto sum = [&](int64_t c, int parts, int at, int step) {
+    f32x8 acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int t = at; t < parts; t += step * U) {
+      f32x8 row[U];
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int64_t i = t + k * kGroups;
-      const int64_t slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
-      row[k] = load8(a.partial + (i < parts ? slot * a.dim + col : 0), i < parts ? valid : 0);
+      for (int k = 0; k < U; ++k) {
+        const int s = t + k * step;
+        const int64_t slot = s == 0 ? 2 * c + 1 : 2 * (c + s);
+        row[k] = load8(a.partial + (s < parts ? slot * a.dim + col : 0), s < parts ? valid : 0);
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) acc += row[k];
     }
-#pragma unroll
-    for (int k = 0; k < U; ++k) acc += row[k];
+    return acc;
+  };
+  if (group < kJoinChunks) {
+    const int parts = parts_of[group];
+    if (parts > 0 && parts <= kJoinAlone) put_row(a, token_of[group], col, sum(c0 + group, parts, 0, 1), valid);
   }
-  part[threadIdx.x] = acc;
-  __syncthreads();
-  if (group != 0 || valid == 0) return;
-  for (int g = 1; g < kGroups; ++g) acc += part[g * G + lane];
-  put_row(a, token, col, acc, valid);
+  for (int i = 0; i < kJoinChunks; ++i) {
+    const int parts = parts_of[i];
+    if (parts <= kJoinAlone) continue;   // (the same for all threads of the block)
+    f32x8 acc = sum(c0 + i, parts, group, kGroups);
+    sums[threadIdx.x] = acc;
+    __syncthreads();
+    if (group == 0 && valid > 0) {
+      for (int g = 1; g < kGroups; ++g) acc += sums[g * G + lane];
+      put_row(a, token_of[i], col, acc, valid);
+    }
+    __syncthreads();
+  }
 }
 
 inline size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
 
+// Whether the two bucket kernels sort the batch, and with which buckets.  Kernel times in us against the radix
+// sort's (keys, passes, row_start), ids of a power law out of 50 000: 8 192 ids 12 / 25, 32 768 17 / 28, 131 072
+// 35 / 37, 524 288 122 / 52 (the block of the most frequent token's bucket takes the longest: a power law puts
+// a tenth of the ids into it); out of 262 144: 15 / 34, 16 / 40, 36 / 51, 115 / 70.
+struct BucketPlan {
+  bool use;
+  int bits, shift;   // 2^bits buckets of 2^shift tokens
+  int64_t tiles, buckets;
+};
+
+BucketPlan plan_buckets(int64_t n, int64_t num_rows) {
+  BucketPlan b;
+  const int bits = ilog2_ceil(static_cast<uint64_t>(num_rows));
+  b.bits = bits - kMaxShift < kMinBucketBits ? kMinBucketBits : bits - kMaxShift;
+  b.shift = bits - b.bits < 0 ? 0 : bits - b.bits;
+  b.tiles = ceil_div(n, kTileIds);
+  b.buckets = ceil_div(num_rows, int64_t(1) << b.shift);
+  b.use = b.bits <= kMaxBucketBits && b.tiles <= kTiles;
+  return b;
+}
+
 struct GradWs {
-  void* sort;
+  void* sort;         // radix sort
   size_t sort_bytes;
   int64_t* keys;
+  uint32_t* tile_tok; // bucket kernels
+  uint32_t* tile_pos;
+  uint32_t* offsets;
+  uint32_t* perm;
+  uint32_t* token;
   uint32_t* row_start;
   float* partial;
   size_t bytes;
@@ -291,21 +541,60 @@ struct GradWs {
 
 GradWs carve_grad(void* base, int64_t n, int64_t dim, int64_t num_rows) {
   const GradPlan p = plan_grad(n, dim);
-  GradWs w;
+  const BucketPlan b = plan_buckets(n, num_rows);
+  GradWs w = {};
   Carver c(base);
-  w.sort_bytes = round256(sort_ids_workspace_bytes(n));
-  w.sort = c.take<char>(w.sort_bytes);
-  w.keys = c.take<int64_t>(n);
+  if (b.use) {
+    w.tile_tok = c.take<uint32_t>(b.tiles * kTileIds);
+    w.tile_pos = c.take<uint32_t>(b.tiles * kTileIds);
+    w.offsets = c.take<uint32_t>(((int64_t(1) << b.bits) + 1) * b.tiles);
+    w.perm = c.take<uint32_t>(n);
+    w.token = c.take<uint32_t>(n);
+  } else {
+    w.sort_bytes = round256(sort_ids_workspace_bytes(n));
+    w.sort = c.take<char>(w.sort_bytes);
+    w.keys = c.take<int64_t>(n);
+  }
   w.row_start = c.take<uint32_t>(num_rows + 1);
   w.partial = c.take<float>(2 * p.chunks * dim);
   w.bytes = c.total();
   return w;
 }
 
+// positions in token order, their tokens, and row_start
+template <typename I>
+int sort_tokens(const I* ids, int64_t n, int64_t rows, int64_t num_rows, int64_t padding, const GradWs& w,
+                const uint32_t** perm, const uint32_t** token, hipStream_t st) {
+  const BucketPlan b = plan_buckets(rows, num_rows);
+  if (b.use) {
+    HADES_LAUNCH((token_tile_kernel<I>), dim3(static_cast<unsigned>(b.tiles)), dim3(kTileIds),
+                 (kTileWaves << b.bits) * sizeof(uint32_t), st, ids, n, num_rows, padding, b.shift, b.bits,
+                 static_cast<int>(b.tiles), w.tile_tok, w.tile_pos, w.offsets);
+    HADES_LAUNCH(token_bucket_kernel, dim3(static_cast<unsigned>(b.buckets)), dim3(kTileIds),
+                 (kTileWaves << b.shift) * sizeof(uint32_t), st, w.tile_tok, w.tile_pos, w.offsets,
+                 static_cast<int>(b.tiles), num_rows, b.shift, w.perm, w.token, w.row_start);
+    *perm = w.perm;
+    *token = w.token;
+    return HADES_OK;
+  }
+  const dim3 block(kThreads);
+  HADES_LAUNCH((token_key_kernel<I>), dim3(static_cast<unsigned>(ceil_div(rows, kThreads))), block, 0, st, ids, n, rows,
+               num_rows, padding, w.keys);
+  SortResult sr;
+  const int rc = sort_ids(w.keys, rows, num_rows + 1, w.sort, w.sort_bytes, st, &sr);
+  if (rc != HADES_OK) return rc;
+  HADES_REQUIRE(!sr.key64, "internal: token keys must be 32-bit");
+  *perm = sr.perm;
+  *token = static_cast<const uint32_t*>(sr.sorted_keys);
+  HADES_LAUNCH(row_start_kernel, dim3(static_cast<unsigned>(ceil_div(num_rows + 1, kThreads))), block, 0, st, *token,
+               rows, num_rows, w.row_start);
+  return HADES_OK;
+}
+
 template <typename T, typename O, int G, int CH>
 int launch_sums(GradArgs<T, O>& a, const GradPlan& p, hipStream_t st) {
   const int64_t sum_blocks = ceil_div(p.chunks * p.slices * G, kThreads);
-  const int64_t zero_blocks = a.accumulate ? 0 : ceil_div(a.zero_pieces, int64_t(kThreads) * kPieces);
+  const int64_t zero_blocks = a.accumulate ? 0 : ceil_div(a.zero_units, int64_t(kThreads) * kZeroUnits);
   HADES_REQUIRE(p.chunks * p.slices < (int64_t(1) << 31) && sum_blocks + zero_blocks < (int64_t(1) << 24) &&
                     p.chunks * p.slices < (int64_t(1) << 24),
                 "embed_grad: too many values for one call");
@@ -313,15 +602,16 @@ int launch_sums(GradArgs<T, O>& a, const GradPlan& p, hipStream_t st) {
   if (sum_blocks + zero_blocks > 0)
     HADES_LAUNCH((embed_grad_sum_kernel<T, O, G, CH>), dim3(static_cast<unsigned>(sum_blocks + zero_blocks)),
                  dim3(kThreads), 0, st, a);
-  if (p.chunks > 1)
-    HADES_LAUNCH((embed_grad_join_kernel<T, O, G, CH>), dim3(static_cast<unsigned>(p.chunks * p.slices)),
-                 dim3(kThreads), 0, st, a);
+  if (p.chunks > 2)   // (no token is longer than two chunks otherwise)
+    HADES_LAUNCH((embed_grad_join_kernel<T, O, G, CH>),
+                 dim3(static_cast<unsigned>(ceil_div(p.chunks, kJoinChunks)), static_cast<unsigned>(p.slices)),
+                 dim3(kJoinThreads), 0, st, a);
   return HADES_OK;
 }
 
 template <typename T, typename O>
 int launch_grad(const void* grad, int64_t grad_stride, const uint32_t* perm, const uint32_t* token, void* out,
-                int64_t out_stride, int64_t num_rows, int64_t dim, const GradPlan& p, const GradWs& w,
+                int64_t out_stride, int64_t n, int64_t num_rows, int64_t dim, const GradPlan& p, const GradWs& w,
                 int accumulate, const DropArgs& drop, hipStream_t st) {
   GradArgs<T, O> a;
   a.grad = static_cast<const T*>(grad);
@@ -337,12 +627,21 @@ int launch_grad(const void* grad, int64_t grad_stride, const uint32_t* perm, con
   a.chunks = p.chunks;
   a.slices = p.slices;
   a.accumulate = accumulate;
-  a.per_row = FastDiv(static_cast<uint32_t>(p.pieces));
+  a.once = streamed(n * dim * static_cast<int64_t>(sizeof(T)));
+  // one more unit where a row may begin inside one
+  constexpr int64_t kUnit = 16 / sizeof(O);
+  const bool aligned = (align_of_ptr(out) & 15) == 0 && out_stride % kUnit == 0;
+  const int64_t units = ceil_div(dim, kUnit) + (aligned ? 0 : 1);
+  a.per_row = FastDiv(static_cast<uint32_t>(units));
   a.per_chunk = FastDiv(static_cast<uint32_t>(p.slices));
-  a.zero_pieces = num_rows * p.pieces;
+  a.zero_units = num_rows * units;
   a.drop = drop;
-#define HADES_SUMS(G_)                                                             \
-  return p.chunk == kLong ? launch_sums<T, O, G_, kLong>(a, p, st) : launch_sums<T, O, G_, kShort>(a, p, st)
+#define HADES_SUMS(G_)                                                   \
+  do {                                                                   \
+    if (p.chunk == kChunkLong) return launch_sums<T, O, G_, kChunkLong>(a, p, st); \
+    if (p.chunk == kChunk) return launch_sums<T, O, G_, kChunk>(a, p, st);         \
+    return launch_sums<T, O, G_, kChunkShort>(a, p, st);                 \
+  } while (0)
   switch (p.group) {
     case 8: HADES_SUMS(8);
     case 16: HADES_SUMS(16);
@@ -413,22 +712,13 @@ int hades_embed_grad(const void* grad, int64_t grad_stride, const void* ids, int
   HADES_REQUIRE((align_of_ptr(workspace) & 255) == 0, "workspace must be 256-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const GradPlan plan = plan_grad(rows, dim);
-  const dim3 block(kThreads), kgrid(static_cast<unsigned>(ceil_div(rows, kThreads)));
-  if (itype == HADES_I64)
-    HADES_LAUNCH((token_key_kernel<int64_t>), kgrid, block, 0, st, static_cast<const int64_t*>(ids), n, rows,
-                 num_rows, padding_idx, w.keys);
-  else
-    HADES_LAUNCH((token_key_kernel<int32_t>), kgrid, block, 0, st, static_cast<const int32_t*>(ids), n, rows,
-                 num_rows, padding_idx, w.keys);
-  SortResult sr;
-  const int rc = sort_ids(w.keys, rows, num_rows + 1, w.sort, w.sort_bytes, st, &sr);
+  const uint32_t *perm = nullptr, *token = nullptr;
+  const int rc = itype == HADES_I64
+                     ? sort_tokens(static_cast<const int64_t*>(ids), n, rows, num_rows, padding_idx, w, &perm, &token, st)
+                     : sort_tokens(static_cast<const int32_t*>(ids), n, rows, num_rows, padding_idx, w, &perm, &token, st);
   if (rc != HADES_OK) return rc;
-  HADES_REQUIRE(!sr.key64, "internal: token keys must be 32-bit");
-  const uint32_t* token = static_cast<const uint32_t*>(sr.sorted_keys);
-  HADES_LAUNCH(row_start_kernel, dim3(static_cast<unsigned>(ceil_div(num_rows + 1, kThreads))), block, 0, st, token,
-               rows, num_rows, w.row_start);
 #define HADES_GRAD(T_, O_)                                                                               \
-  return launch_grad<T_, O_>(grad, grad_stride, sr.perm, token, out, out_stride, num_rows, dim, plan, w, \
+  return launch_grad<T_, O_>(grad, grad_stride, perm, token, out, out_stride, n, num_rows, dim, plan, w, \
                              accumulate != 0, drop, st)
   if (dtype == HADES_F32) HADES_GRAD(float, float);
   if (dtype == HADES_F16) {

@@ -38,6 +38,10 @@ inline bool make_drop(double p, uint64_t seed, int64_t offset, const int64_t* of
   return true;
 }
 
+// Whether rows of this many bytes are read with non-temporal loads: what does not fit the last-level cache (256
+// MB) cannot be there from the kernel before, and would only push other data out of it.
+inline bool streamed(int64_t bytes) { return bytes >= (int64_t(1) << 28); }
+
 // n / d for n < 2^31 as a multiplication (Granlund and Montgomery's round-up form)
 struct FastDiv {
   uint32_t d, mul, shift;
@@ -61,29 +65,34 @@ struct Vec8 {
 };
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
-// p[0 .. 8) (or its first `valid` values, zeros behind them) as float32
+// p[0 .. 8), or its first `valid` values and zeros behind them.  kOnce / kPast: non-temporal, for rows
+// that are read once and values that are not read again soon.
 template <typename T, bool kOnce = false>
-__device__ __forceinline__ f32x8 load8(const T* __restrict__ p, int valid) {
-  if (valid >= kPiece) {
-    typedef typename Vec8<T>::VU VU;
-    const VU v = kOnce ? __builtin_nontemporal_load(reinterpret_cast<const VU*>(p))
-                       : *reinterpret_cast<const VU*>(p);
-    return __builtin_convertvector(v, f32x8);
-  }
-  f32x8 r = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ typename Vec8<T>::V load8_raw(const T* __restrict__ p, int valid) {
+  typedef typename Vec8<T>::VU VU;
+  if (valid >= kPiece)
+    return kOnce ? __builtin_nontemporal_load(reinterpret_cast<const VU*>(p)) : *reinterpret_cast<const VU*>(p);
+  typename Vec8<T>::V r;
 #pragma unroll
-  for (int j = 0; j < kPiece - 1; ++j)
-    if (j < valid) r[j] = static_cast<float>(p[j]);
+  for (int j = 0; j < kPiece; ++j) r[j] = j < valid ? p[j] : static_cast<T>(0.0f);
   return r;
 }
 
+// ... as float32
+template <typename T, bool kOnce = false>
+__device__ __forceinline__ f32x8 load8(const T* __restrict__ p, int valid) {
+  return __builtin_convertvector((load8_raw<T, kOnce>(p, valid)), f32x8);
+}
+
 // rounds to nearest even, once
-template <typename T>
+template <typename T, bool kPast = false>
 __device__ __forceinline__ void store8(T* __restrict__ p, f32x8 v, int valid) {
   if (valid >= kPiece) {
     typedef typename Vec8<T>::V V;
     typedef typename Vec8<T>::VU VU;
-    *reinterpret_cast<VU*>(p) = __builtin_convertvector(v, V);
+    const VU r = __builtin_convertvector(v, V);
+    if (kPast) __builtin_nontemporal_store(r, reinterpret_cast<VU*>(p));
+    else *reinterpret_cast<VU*>(p) = r;
     return;
   }
 #pragma unroll
