@@ -852,16 +852,34 @@ _ID_TYPES = {torch.int32: _lib.I32, torch.int64: _lib.I64}
 _U64 = (1 << 64) - 1
 
 
+_device_of_thread = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _row_type(t, name):
     code = _ROW_TYPES.get(t.dtype)
-    _check(code is not None, "Type can only be float, half or bfloat16 (%s is %s)" % (name, t.dtype))
+    if code is None:
+        raise RuntimeError("Type can only be float, half or bfloat16 (%s is %s)" % (name, t.dtype))
     return code
+
+
+def _enter(t, name):
+    """(device, its current stream) of a call whose first tensor is t."""
+    if not t.is_cuda:
+        raise RuntimeError("%s must be a device tensor" % name)
+    dev = t.device
+    if dev.index != _device_of_thread():
+        raise RuntimeError("%s is on %s, which is not the current device: launches go to the current device's "
+                           "stream" % (name, dev))
+    return dev, _raw_stream(dev.index)
 
 
 def _row_stride(t, name, device):
     """Elements between the rows of t (its last dimension), which lies on `device`."""
-    _check(t.is_cuda and t.device == device, "%s must be a device tensor on %s" % (name, device))
-    _check(t.dim() >= 1, "%s must have at least one dimension" % name)
+    if t.device != device:
+        raise RuntimeError("%s must be a device tensor on %s" % (name, device))
+    if t.dim() == 0:
+        raise RuntimeError("%s must have at least one dimension" % name)
     cols = t.size(-1)
     if t.is_contiguous() or t.numel() == 0:
         return cols
@@ -874,52 +892,65 @@ def _row_stride(t, name, device):
     return v.stride(0) if v.size(0) > 1 else cols
 
 
-def _current(t, name):
-    _check(t.is_cuda, "%s must be a device tensor" % name)
-    _check(t.device.index == torch.cuda.current_device(),
-           "%s is on %s, which is not the current device: launches go to the current device's stream"
-           % (name, t.device))
-    return t.device
+def _ids_type(ids, device):
+    code = _ID_TYPES.get(ids.dtype)
+    if code is None:
+        raise RuntimeError("ID can only be int32 or int64 (ids is %s)" % ids.dtype)
+    if ids.device != device or not ids.is_contiguous():
+        raise RuntimeError("ids must be a contiguous tensor on %s" % device)
+    return code
+
+
+_NO_DROP = (0.0, 0, 0, None)
 
 
 def _drop_args(dropout, device):
+    """p, seed, offset, offset pointer of the C ABI"""
     if dropout is None:
-        return 0.0, 0, 0, _NULL
+        return _NO_DROP
     p, seed, offset = dropout
     _check(0.0 <= p <= 1.0, "dropout: p must lie in [0, 1]")
-    ptr = _NULL
+    ptr = None
     if isinstance(offset, torch.Tensor):
         _check(offset.dtype == torch.int64 and offset.numel() == 1 and offset.device == device,
                "dropout: offset must be an int or an int64 tensor of one element on the device")
-        ptr, offset = _ptr(offset), 0
+        ptr, offset = offset.data_ptr(), 0
     _check(-(1 << 63) <= seed <= _U64 and 0 <= offset < (1 << 63),
            "dropout: seed must fit 64 bits, offset must be in [0, 2^63)")
     return float(p), seed & _U64, offset, ptr
 
 
-def _dense_out(out, shape, dtype, device, name="out"):
+def _out_like(x, dtype, out, name="out"):
+    """A dense tensor of x's shape and of dtype: `out` after its checks, or a new one."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    _check(out.device == device and out.is_contiguous(), "%s must be a contiguous tensor on %s" % (name, device))
-    _check(tuple(out.shape) == tuple(shape) and out.dtype == dtype, "%s has the wrong shape/dtype" % name)
+        return torch.empty_like(x) if x.dtype == dtype and x.is_contiguous() else x.new_empty(x.shape, dtype=dtype)
+    _check(out.device == x.device and out.is_contiguous(), "%s must be a contiguous tensor on %s" % (name, x.device))
+    _check(out.shape == x.shape and out.dtype == dtype, "%s has the wrong shape/dtype" % name)
     return out
+
+
+def _ptr_or_none(t):
+    return None if t is None else t.data_ptr()
 
 
 def embed(weight, ids, scale=1.0, dropout=None, out=None):
     """out[..., :] = scale * weight[ids[...], :], then dropout; rows of the table's type, of shape
     ids.shape + (dim,).  weight [num_rows, dim] may be a row-strided view; ids int32 or int64.  An
     id outside [0, num_rows) (padding, e.g. -1) gives a row of zeros."""
-    dev = _current(weight, "weight")
+    dev, stream = _enter(weight, "weight")
     _check(weight.dim() == 2 and weight.size(1) >= 1, "weight must be [num_rows, dim]")
     dtype, stride = _row_type(weight, "weight"), _row_stride(weight, "weight", dev)
-    itype = _ID_TYPES.get(ids.dtype)
-    _check(itype is not None, "ID can only be int32 or int64 (ids is %s)" % ids.dtype)
-    _check(ids.device == dev and ids.is_contiguous(), "ids must be a contiguous tensor on %s" % dev)
+    itype = _ids_type(ids, dev)
     drop = _drop_args(dropout, dev)
-    dim = weight.size(1)
-    out = _dense_out(out, (*ids.shape, dim), weight.dtype, dev)
-    _lib.call("hades_embed", _ptr(weight), stride, weight.size(0), _ptr(ids), ids.numel(), _ptr(out), dim, dtype,
-              itype, float(scale), *drop, _stream())
+    num_rows, dim = weight.shape
+    shape = (*ids.shape, dim)
+    if out is None:
+        out = weight.new_empty(shape)
+    else:
+        _check(out.device == dev and out.is_contiguous(), "out must be a contiguous tensor on %s" % dev)
+        _check(out.shape == shape and out.dtype == weight.dtype, "out has the wrong shape/dtype")
+    _lib.call("hades_embed", weight.data_ptr(), stride, num_rows, ids.data_ptr(), ids.numel(), out.data_ptr(), dim,
+              dtype, itype, scale, *drop, stream)
     return out
 
 
@@ -930,44 +961,43 @@ def embed_grad(grad, ids, num_rows, scale=1.0, padding_idx=None, dropout=None, o
     run.  Tokens that do not occur get rows of zeros.  `accumulate` adds to `out` instead and leaves the
     rows of absent tokens alone.  Ids outside [0, num_rows) and `padding_idx` have no gradient.  `out`
     ([num_rows, dim], may be row-strided) has grad's type or float32, as has `out_dtype`."""
-    dev = _current(grad, "grad")
+    dev, stream = _enter(grad, "grad")
     dtype, stride = _row_type(grad, "grad"), _row_stride(grad, "grad", dev)
     dim, n = grad.size(-1), ids.numel()
-    itype = _ID_TYPES.get(ids.dtype)
-    _check(itype is not None, "ID can only be int32 or int64 (ids is %s)" % ids.dtype)
-    _check(ids.device == dev and ids.is_contiguous(), "ids must be a contiguous tensor on %s" % dev)
+    itype = _ids_type(ids, dev)
     _check(dim >= 1 and grad.numel() == n * dim, "grad must have one row per id")
     _check(num_rows >= 0, "num_rows must be >= 0")
     _check(padding_idx is None or 0 <= padding_idx < num_rows, "padding_idx must be in [0, num_rows)")
     drop = _drop_args(dropout, dev)
     if out is None:
         _check(not accumulate, "accumulate needs out")
-        out = torch.empty((num_rows, dim), dtype=out_dtype or grad.dtype, device=dev)
-    _check(out.dim() == 2 and tuple(out.shape) == (num_rows, dim) and out_dtype in (None, out.dtype),
-           "out has the wrong shape/dtype")
-    _check(out.dtype in (grad.dtype, torch.float32), "the gradient's type is the rows' or float")
-    ws = torch.empty(_lib.query("hades_embed_grad_workspace_bytes", n, dim, num_rows), dtype=torch.uint8, device=dev)
-    _lib.call("hades_embed_grad", _ptr(grad), stride, _ptr(ids), n, _ptr(out), _row_stride(out, "out", dev), num_rows,
-              dim, dtype, _ROW_TYPES[out.dtype], itype, -1 if padding_idx is None else int(padding_idx),
-              int(bool(accumulate)), float(scale), *drop, _ptr(ws), ws.numel(), _stream())
+        out = grad.new_empty((num_rows, dim), dtype=out_dtype)
+    _check(out.shape == (num_rows, dim) and out_dtype in (None, out.dtype), "out has the wrong shape/dtype")
+    _check(out.dtype == grad.dtype or out.dtype == torch.float32, "the gradient's type is the rows' or float")
+    nbytes = _lib.query("hades_embed_grad_workspace_bytes", n, dim, num_rows)
+    ws = grad.new_empty(nbytes, dtype=torch.uint8)
+    _lib.call("hades_embed_grad", grad.data_ptr(), stride, ids.data_ptr(), n, out.data_ptr(),
+              _row_stride(out, "out", dev), num_rows, dim, dtype, _ROW_TYPES[out.dtype], itype,
+              -1 if padding_idx is None else padding_idx, bool(accumulate), scale, *drop, ws.data_ptr(), nbytes, stream)
     return out
 
 
 def dropout(x, p, seed, offset, residual=None, out=None):
     """out = x with a share p of its values zeroed and the others divided by 1 - p, plus `residual` (of
     x's shape and type).  `out` may be x or residual."""
-    dev = _current(x, "x")
+    dev, stream = _enter(x, "x")
     dtype, stride = _row_type(x, "x"), _row_stride(x, "x", dev)
     res_stride = 0
     if residual is not None:
         _check(residual.shape == x.shape and residual.dtype == x.dtype, "residual must have x's shape and dtype")
         res_stride = _row_stride(residual, "residual", dev)
     drop = _drop_args((p, seed, offset), dev)
-    out = _dense_out(out, x.shape, x.dtype, dev)
-    if out.numel():
+    out = _out_like(x, x.dtype, out)
+    n = out.numel()
+    if n:
         cols = x.size(-1)
-        _lib.call("hades_dropout", _ptr(x), stride, _opt(residual), res_stride, _ptr(out), x.numel() // cols, cols,
-                  dtype, *drop, _stream())
+        _lib.call("hades_dropout", x.data_ptr(), stride, _ptr_or_none(residual), res_stride, out.data_ptr(), n // cols,
+                  cols, dtype, *drop, stream)
     return out
 
 
@@ -977,20 +1007,32 @@ def dropout_grad(grad, p, seed, offset, out=None):
     return dropout(grad, p, seed, offset, out=out)
 
 
-def _norm_args(x, weight, residual, dropout, dev):
-    dtype = _row_type(x, "x")
-    _check(x.dim() >= 1 and x.size(-1) >= 1, "x must have rows of at least one value")
-    stream_type, res_stride, weight_type = x.dtype, 0, dtype
+def _weight_type(weight, x, cols, name):
+    """C type of a norm's weight beside rows x"""
+    if (weight.device != x.device or weight.dim() != 1 or weight.size(0) != cols or not weight.is_contiguous()
+            or (weight.dtype != x.dtype and weight.dtype != torch.float32)):
+        raise RuntimeError("weight must be contiguous [columns of %s] on %s, of %s's dtype or float32"
+                           % (name, x.device, name))
+    return _ROW_TYPES[weight.dtype]
+
+
+def _norm_args(x, weight, residual, dropout, dev, h_out):
+    """(type, row stride, columns, residual's stride, weight's type, dropout, h) of a norm's forward call"""
+    dtype, stride = _row_type(x, "x"), _row_stride(x, "x", dev)
+    cols = x.size(-1)
+    _check(cols >= 1, "x must have rows of at least one value")
+    h_dtype, res_stride, weight_type = x.dtype, 0, dtype
     if residual is not None:
-        _check(residual.shape == x.shape and residual.dtype in (x.dtype, torch.float32),
+        h_dtype = residual.dtype
+        _check(residual.shape == x.shape and (h_dtype == x.dtype or h_dtype == torch.float32),
                "residual must have x's shape, and x's dtype or float32")
-        stream_type, res_stride = residual.dtype, _row_stride(residual, "residual", dev)
+        res_stride = _row_stride(residual, "residual", dev)
     if weight is not None:
-        _check(weight.device == dev and tuple(weight.shape) == (x.size(-1),) and weight.is_contiguous()
-               and weight.dtype in (x.dtype, torch.float32),
-               "weight must be contiguous [columns of x] on %s, of x's dtype or float32" % dev)
-        weight_type = _ROW_TYPES[weight.dtype]
-    return dtype, stream_type, res_stride, weight_type, _drop_args(dropout, dev)
+        weight_type = _weight_type(weight, x, cols, "x")
+    h = x
+    if residual is not None or dropout is not None or h_out is not None:
+        h = _out_like(x, h_dtype, h_out, "h_out")
+    return dtype, stride, cols, res_stride, weight_type, _drop_args(dropout, dev), h
 
 
 def rms_norm(x, weight=None, eps=1e-6, residual=None, dropout=None, out=None, h_out=None):
@@ -999,17 +1041,13 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, dropout=None, out=None, h_
     nor dropout), rstd = 1 / sqrt(...) float32 of shape x.shape[:-1], for rms_norm_grad.  The norm is
     taken of h before its rounding.  residual and weight have x's type or float32; weight None: ones.
     `h_out` may be residual."""
-    dev = _current(x, "x")
-    dtype, stream_type, res_stride, weight_type, drop = _norm_args(x, weight, residual, dropout, dev)
-    stride, cols = _row_stride(x, "x", dev), x.size(-1)
-    y = _dense_out(out, x.shape, x.dtype, dev)
-    h = x
-    if residual is not None or dropout is not None or h_out is not None:
-        h = _dense_out(h_out, x.shape, stream_type, dev, "h_out")
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    _lib.call("hades_rms_norm", _ptr(x), stride, _opt(residual), res_stride, _opt(weight), _ptr(y), _NULL,
-              _NULL if h is x else _ptr(h), _ptr(rstd), rstd.numel(), cols, dtype, _ROW_TYPES[stream_type],
-              weight_type, 0, float(eps), *drop, _stream())
+    dev, stream = _enter(x, "x")
+    dtype, stride, cols, res_stride, weight_type, drop, h = _norm_args(x, weight, residual, dropout, dev, h_out)
+    y = _out_like(x, x.dtype, out)
+    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    _lib.call("hades_rms_norm", x.data_ptr(), stride, _ptr_or_none(residual), res_stride, _ptr_or_none(weight),
+              y.data_ptr(), None, None if h is x else h.data_ptr(), rstd.data_ptr(), rstd.numel(), cols, dtype,
+              _ROW_TYPES[h.dtype], weight_type, 0, eps, *drop, stream)
     return y, h, rstd
 
 
@@ -1018,20 +1056,16 @@ def rms_norm_8bit(x, weight=None, eps=1e-6, residual=None, group=0, dropout=None
     h).  y is about q * scale, with one scale for every `group` columns (a power of two from 8 to 512; 0:
     one for the row), scale = max|y| / 448.  A group of zeros has scale 0; one with an infinity or a NaN
     has a scale that is one too."""
-    dev = _current(x, "x")
-    dtype, stream_type, res_stride, weight_type, drop = _norm_args(x, weight, residual, dropout, dev)
-    stride, cols = _row_stride(x, "x", dev), x.size(-1)
+    dev, stream = _enter(x, "x")
+    dtype, stride, cols, res_stride, weight_type, drop, h = _norm_args(x, weight, residual, dropout, dev, h_out)
     _check(group == 0 or (8 <= group <= 512 and group & (group - 1) == 0),
            "group must be 0 or a power of two in [8, 512]")
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
     groups = 1 if group == 0 else -(-cols // group)
-    scales = torch.empty((*x.shape[:-1], groups), dtype=torch.float32, device=dev)
-    h = x
-    if residual is not None or dropout is not None or h_out is not None:
-        h = _dense_out(h_out, x.shape, stream_type, dev, "h_out")
-    _lib.call("hades_rms_norm", _ptr(x), stride, _opt(residual), res_stride, _opt(weight), _ptr(q), _ptr(scales),
-              _NULL if h is x else _ptr(h), _NULL, scales.numel() // groups, cols, dtype, _ROW_TYPES[stream_type],
-              weight_type, int(group), float(eps), *drop, _stream())
+    scales = x.new_empty((*x.shape[:-1], groups), dtype=torch.float32)
+    _lib.call("hades_rms_norm", x.data_ptr(), stride, _ptr_or_none(residual), res_stride, _ptr_or_none(weight),
+              q.data_ptr(), scales.data_ptr(), None if h is x else h.data_ptr(), None, scales.numel() // groups, cols,
+              dtype, _ROW_TYPES[h.dtype], weight_type, group, eps, *drop, stream)
     return q, scales, h
 
 
@@ -1041,34 +1075,31 @@ def rms_norm_grad(grad, h, weight, rstd, grad_h=None, dropout=None, weight_grad=
     grad_residual h's; where the two have the same values and type they are one tensor.  grad_weight
     (weight's type, summed in float32 in a fixed order) is None without weight or weight_grad,
     grad_residual None without residual_grad."""
-    dev = _current(grad, "grad")
-    dtype = _row_type(grad, "grad")
-    _check(grad.dim() >= 1 and grad.size(-1) >= 1, "grad must have rows of at least one value")
+    dev, stream = _enter(grad, "grad")
+    dtype, grad_stride = _row_type(grad, "grad"), _row_stride(grad, "grad", dev)
     cols = grad.size(-1)
-    _check(h.shape == grad.shape and h.dtype in (grad.dtype, torch.float32),
+    _check(cols >= 1, "grad must have rows of at least one value")
+    _check(h.shape == grad.shape and (h.dtype == grad.dtype or h.dtype == torch.float32),
            "h must have grad's shape, and grad's dtype or float32")
     _check(grad_h is None or (grad_h.shape == h.shape and grad_h.dtype == h.dtype),
            "grad_h must have h's shape and dtype")
     _check(rstd.device == dev and rstd.dtype == torch.float32 and rstd.is_contiguous()
            and rstd.shape == grad.shape[:-1], "rstd must be the contiguous float32 tensor that rms_norm returned")
-    weight_type = dtype
-    if weight is not None:
-        _check(weight.device == dev and tuple(weight.shape) == (cols,) and weight.is_contiguous()
-               and weight.dtype in (grad.dtype, torch.float32),
-               "weight must be contiguous [columns of grad] on %s, of grad's dtype or float32" % dev)
-        weight_type = _ROW_TYPES[weight.dtype]
+    weight_type = dtype if weight is None else _weight_type(weight, grad, cols, "grad")
     drop = _drop_args(dropout, dev)
-    grad_stride, h_stride = _row_stride(grad, "grad", dev), _row_stride(h, "h", dev)
+    h_stride = _row_stride(h, "h", dev)
     gh_stride = 0 if grad_h is None else _row_stride(grad_h, "grad_h", dev)
-    grad_x = torch.empty(grad.shape, dtype=grad.dtype, device=dev)
+    grad_x = _out_like(grad, grad.dtype, None)
     apart = residual_grad and (dropout is not None or h.dtype != grad.dtype)
-    grad_res = torch.empty(grad.shape, dtype=h.dtype, device=dev) if apart else None
+    grad_res = _out_like(grad, h.dtype, None) if apart else None
+    rows, nbytes = rstd.numel(), 0
     grad_w = ws = None
     if weight is not None and weight_grad:
         grad_w = torch.empty_like(weight)
-        ws = torch.empty(_lib.query("hades_rms_norm_grad_workspace_bytes", rstd.numel(), cols), dtype=torch.uint8,
-                         device=dev)
-    _lib.call("hades_rms_norm_grad", _ptr(grad), grad_stride, _ptr(h), h_stride, _opt(weight), _ptr(rstd),
-              _opt(grad_h), gh_stride, _ptr(grad_x), _opt(grad_res), _opt(grad_w), rstd.numel(), cols, dtype,
-              _ROW_TYPES[h.dtype], weight_type, *drop, _opt(ws), 0 if ws is None else ws.numel(), _stream())
+        nbytes = _lib.query("hades_rms_norm_grad_workspace_bytes", rows, cols)
+        ws = grad.new_empty(nbytes, dtype=torch.uint8)
+    _lib.call("hades_rms_norm_grad", grad.data_ptr(), grad_stride, h.data_ptr(), h_stride, _ptr_or_none(weight),
+              rstd.data_ptr(), _ptr_or_none(grad_h), gh_stride, grad_x.data_ptr(), _ptr_or_none(grad_res),
+              _ptr_or_none(grad_w), rows, cols, dtype, _ROW_TYPES[h.dtype], weight_type, *drop, _ptr_or_none(ws),
+              nbytes, stream)
     return grad_x, (grad_res if apart else grad_x) if residual_grad else None, grad_w
