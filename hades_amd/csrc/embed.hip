@@ -259,6 +259,53 @@ __global__ __launch_bounds__(kTileIds) void token_bucket_kernel(const uint32_t* 
   }
 }
 
+// A batch of one tile without the first kernel: the block of a bucket looks at all ids itself.
+template <typename I>
+__global__ __launch_bounds__(kTileIds) void token_small_kernel(const I* __restrict__ ids, int64_t n, int64_t num_rows,
+                                                               int64_t padding, int shift, uint32_t* __restrict__ perm,
+                                                               uint32_t* __restrict__ token,
+                                                               uint32_t* __restrict__ row_start) {
+  extern __shared__ uint32_t counts[];   // [kTileWaves][2^shift]
+  __shared__ uint32_t scan[kTileWaves + 1];
+  const int range = 1 << shift;
+  const uint32_t v0 = blockIdx.x << shift;
+  const uint32_t rows = static_cast<uint32_t>(num_rows);
+  const uint32_t mine = rows - v0 < static_cast<uint32_t>(range) ? rows - v0 : static_cast<uint32_t>(range);
+  const int wave = threadIdx.x / kWave;
+  const int64_t id = threadIdx.x < n ? static_cast<int64_t>(ids[threadIdx.x]) : int64_t(-1);
+  const bool real = static_cast<uint64_t>(id) < static_cast<uint64_t>(num_rows) && id != padding;
+  const uint32_t at = static_cast<uint32_t>(id) - v0;
+  const bool in = real && at < mine;
+  for (int k = threadIdx.x; k < kTileWaves * range; k += kTileIds) counts[k] = 0;
+  uint32_t base;   // tokens below the range
+  block_exclusive_sum<uint32_t, kTileIds>(real && static_cast<uint32_t>(id) < v0 ? 1u : 0u, scan, &base);
+  const uint64_t peers = peers_of(in ? at : 0u, shift, __ballot(in));
+  const uint32_t rank = ballot_rank(peers);
+  if (in && rank == 0) counts[wave * range + at] = static_cast<uint32_t>(__popcll(peers));
+  __syncthreads();
+  uint32_t total = 0;
+  if (threadIdx.x < mine) {
+    for (int w = 0; w < kTileWaves; ++w) {
+      const uint32_t c = counts[w * range + threadIdx.x];
+      counts[w * range + threadIdx.x] = total;
+      total += c;
+    }
+  }
+  uint32_t all;
+  const uint32_t start = base + block_exclusive_sum<uint32_t, kTileIds>(total, scan, &all);
+  if (threadIdx.x < mine) {
+    row_start[v0 + threadIdx.x] = start;
+    for (int w = 0; w < kTileWaves; ++w) counts[w * range + threadIdx.x] += start;
+  }
+  if (v0 + mine == rows && threadIdx.x == 0) row_start[rows] = base + all;
+  __syncthreads();
+  if (in) {
+    const uint32_t to = counts[wave * range + at] + rank;
+    perm[to] = threadIdx.x;
+    token[to] = static_cast<uint32_t>(id);
+  }
+}
+
 // row_start[v] = number of sorted tokens below v, for v in [0, num_rows]
 __global__ __launch_bounds__(kThreads) void row_start_kernel(const uint32_t* __restrict__ token, int64_t n,
                                                              int64_t num_rows, uint32_t* __restrict__ row_start) {
@@ -309,8 +356,8 @@ struct GradArgs {
   const uint32_t* token;       // its token
   const uint32_t* row_start;   // [num_rows + 1]
   O* out;
-  float* partial;              // [2 * chunks][dim], see is_long
-  int64_t grad_stride, out_stride, num_rows, dim, chunks;
+  float* partial;              // [2 * chunks][partial_stride], see is_long
+  int64_t grad_stride, out_stride, partial_stride, num_rows, dim, chunks;
   int slices, accumulate;
   int once;                    // rows of grad: see streamed
   unsigned sum_blocks;
@@ -394,7 +441,7 @@ __global__ __launch_bounds__(kThreads) void embed_grad_sum_kernel(GradArgs<T, O>
   const f32x8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   f32x8 acc = zero;
   // slot 0: a long token that began earlier; slot 1: one that begins here
-  float* const slot = a.partial + 2 * static_cast<int64_t>(chunk) * a.dim + col;
+  float* const slot = a.partial + 2 * static_cast<int64_t>(chunk) * a.partial_stride + col;
   const int len = static_cast<int>(p1 - p0);
   for (int t = 0; t < len; t += U) {
     typename Vec8<T>::V row[U];
@@ -418,7 +465,7 @@ __global__ __launch_bounds__(kThreads) void embed_grad_sum_kernel(GradArgs<T, O>
     for (int k = 0; k < U; ++k) {
       if (t + k >= len) break;
       if (tok[k] != cur) {
-        if (part) store8(slot, acc, valid);   // (only the chunk's first token can end here as a long one)
+        if (part) store8(slot, acc, kPiece);   // (only the chunk's first token can end here as a long one)
         else put_row(a, cur, col, acc, valid);
         acc = zero;
         cur = tok[k];
@@ -430,7 +477,7 @@ __global__ __launch_bounds__(kThreads) void embed_grad_sum_kernel(GradArgs<T, O>
   }
   if (part || (cur == last && is_long<CH>(last_begin, last_end))) {
     const bool begins = static_cast<int64_t>(a.row_start[cur]) >= static_cast<int64_t>(chunk) * CH;
-    store8(slot + (begins ? a.dim : 0), acc, valid);
+    store8(slot + (begins ? a.partial_stride : 0), acc, kPiece);
   } else {
     put_row(a, cur, col, acc, valid);
   }
@@ -477,7 +524,7 @@ __global__ __launch_bounds__(kJoinThreads) void embed_grad_join_kernel(GradArgs<
       for (int k = 0; k < U; ++k) {
         const int s = t + k * step;
         const int64_t slot = s == 0 ? 2 * c + 1 : 2 * (c + s);
-        row[k] = load8(a.partial + (s < parts ? slot * a.dim + col : 0), s < parts ? valid : 0);
+        row[k] = load8(a.partial + (s < parts ? slot * a.partial_stride + col : 0), s < parts && valid > 0 ? kPiece : 0);
       }
 #pragma unroll
       for (int k = 0; k < U; ++k) acc += row[k];
@@ -556,7 +603,7 @@ GradWs carve_grad(void* base, int64_t n, int64_t dim, int64_t num_rows) {
     w.keys = c.take<int64_t>(n);
   }
   w.row_start = c.take<uint32_t>(num_rows + 1);
-  w.partial = c.take<float>(2 * p.chunks * dim);
+  w.partial = c.take<float>(2 * p.chunks * p.pieces * kPiece);
   w.bytes = c.total();
   return w;
 }
@@ -566,6 +613,14 @@ template <typename I>
 int sort_tokens(const I* ids, int64_t n, int64_t rows, int64_t num_rows, int64_t padding, const GradWs& w,
                 const uint32_t** perm, const uint32_t** token, hipStream_t st) {
   const BucketPlan b = plan_buckets(rows, num_rows);
+  if (b.use && b.tiles == 1) {
+    HADES_LAUNCH((token_small_kernel<I>), dim3(static_cast<unsigned>(b.buckets)), dim3(kTileIds),
+                 (kTileWaves << b.shift) * sizeof(uint32_t), st, ids, n, num_rows, padding, b.shift, w.perm, w.token,
+                 w.row_start);
+    *perm = w.perm;
+    *token = w.token;
+    return HADES_OK;
+  }
   if (b.use) {
     HADES_LAUNCH((token_tile_kernel<I>), dim3(static_cast<unsigned>(b.tiles)), dim3(kTileIds),
                  (kTileWaves << b.bits) * sizeof(uint32_t), st, ids, n, num_rows, padding, b.shift, b.bits,
@@ -625,6 +680,7 @@ int launch_grad(const void* grad, int64_t grad_stride, const uint32_t* perm, con
   a.num_rows = num_rows;
   a.dim = dim;
   a.chunks = p.chunks;
+  a.partial_stride = p.pieces * kPiece;   // whole pieces: aligned whatever dim is
   a.slices = p.slices;
   a.accumulate = accumulate;
   a.once = streamed(n * dim * static_cast<int64_t>(sizeof(T)));
