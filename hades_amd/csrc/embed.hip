@@ -333,6 +333,7 @@ struct GradPlan {
   int group;        // lanes that walk a chunk's rows together: 8, 16, 32 or 64
   int slices;       // groups side by side along a row
   int chunk;
+  int reach;        // chunks that a token may touch before it is a long one
   int64_t chunks;
   int64_t pieces;   // of a row
 };
@@ -346,6 +347,8 @@ GradPlan plan_grad(int64_t n, int64_t dim) {
   const auto waves = [&](int chunk) { return ceil_div(ceil_div(n, chunk) * p.slices * p.group, kWave); };
   p.chunk = waves(kChunkLong) >= kChunkLongWaves ? kChunkLong : (waves(kChunk) >= kChunkWaves ? kChunk : kChunkShort);
   p.chunks = ceil_div(n, p.chunk);
+  // a batch of up to 64 positions has no long tokens and needs no join
+  p.reach = p.chunks <= 8 && p.chunk == kChunkShort ? 8 : 2;
   return p;
 }
 
@@ -358,7 +361,7 @@ struct GradArgs {
   O* out;
   float* partial;              // [2 * chunks][partial_stride], see is_long
   int64_t grad_stride, out_stride, partial_stride, num_rows, dim, chunks;
-  int slices, accumulate;
+  int slices, accumulate, reach;
   int once;                    // rows of grad: see streamed
   unsigned sum_blocks;
   FastDiv per_row, per_chunk;
@@ -373,9 +376,9 @@ __device__ __forceinline__ void put_row(const GradArgs<T, O>& a, uint32_t token,
   store8(p, v, valid);
 }
 
-// a token whose rows reach beyond the chunk behind the one that it begins in
+// a token whose rows reach beyond `reach` chunks, the one that it begins in among them
 template <int CH>
-__device__ __forceinline__ bool is_long(int64_t begin, int64_t end) { return end > (begin / CH + 2) * CH; }
+__device__ __forceinline__ bool is_long(int64_t begin, int64_t end, int reach) { return end > (begin / CH + reach) * CH; }
 
 template <typename T, typename O, int G, int CH>
 __global__ __launch_bounds__(kThreads) void embed_grad_sum_kernel(GradArgs<T, O> a) {
@@ -429,13 +432,13 @@ __global__ __launch_bounds__(kThreads) void embed_grad_sum_kernel(GradArgs<T, O>
   bool part = false;   // the token summed now is a long one: its row is partial
   {
     const int64_t begin = a.row_start[cur], end = a.row_start[cur + 1];
-    if (is_long<CH>(begin, end)) part = true;
+    if (is_long<CH>(begin, end, a.reach)) part = true;
     else if (begin < p0) p0 = end;
   }
   // ... and the last one goes on behind it: taken to its end, unless it is long
   const uint32_t last = a.token[p1 - 1];
   const int64_t last_begin = a.row_start[last], last_end = a.row_start[last + 1];
-  if (last_begin >= static_cast<int64_t>(chunk) * CH && !is_long<CH>(last_begin, last_end)) p1 = last_end;
+  if (last_begin >= static_cast<int64_t>(chunk) * CH && !is_long<CH>(last_begin, last_end, a.reach)) p1 = last_end;
   if (p0 >= p1) return;
   cur = a.token[p0];
   const f32x8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -475,7 +478,7 @@ __global__ __launch_bounds__(kThreads) void embed_grad_sum_kernel(GradArgs<T, O>
       acc += keys.on() ? keys.apply(v, pos[k], piece) : v * keys.factor;
     }
   }
-  if (part || (cur == last && is_long<CH>(last_begin, last_end))) {
+  if (part || (cur == last && is_long<CH>(last_begin, last_end, a.reach))) {
     const bool begins = static_cast<int64_t>(a.row_start[cur]) >= static_cast<int64_t>(chunk) * CH;
     store8(slot + (begins ? a.partial_stride : 0), acc, kPiece);
   } else {
@@ -505,7 +508,7 @@ __global__ __launch_bounds__(kJoinThreads) void embed_grad_join_kernel(GradArgs<
     if (border < live) {
       const uint32_t token = a.token[border - 1];
       const int64_t begin = a.row_start[token], end = a.row_start[token + 1];
-      if (begin >= c * CH && is_long<CH>(begin, end)) parts = static_cast<int>((end - 1) / CH - c + 1);
+      if (begin >= c * CH && is_long<CH>(begin, end, a.reach)) parts = static_cast<int>((end - 1) / CH - c + 1);
       token_of[threadIdx.x] = token;
     }
     parts_of[threadIdx.x] = parts;
@@ -657,7 +660,7 @@ int launch_sums(GradArgs<T, O>& a, const GradPlan& p, hipStream_t st) {
   if (sum_blocks + zero_blocks > 0)
     HADES_LAUNCH((embed_grad_sum_kernel<T, O, G, CH>), dim3(static_cast<unsigned>(sum_blocks + zero_blocks)),
                  dim3(kThreads), 0, st, a);
-  if (p.chunks > 2)   // (no token is longer than two chunks otherwise)
+  if (p.chunks > p.reach)   // (there are no long tokens otherwise)
     HADES_LAUNCH((embed_grad_join_kernel<T, O, G, CH>),
                  dim3(static_cast<unsigned>(ceil_div(p.chunks, kJoinChunks)), static_cast<unsigned>(p.slices)),
                  dim3(kJoinThreads), 0, st, a);
@@ -682,6 +685,7 @@ int launch_grad(const void* grad, int64_t grad_stride, const uint32_t* perm, con
   a.chunks = p.chunks;
   a.partial_stride = p.pieces * kPiece;   // whole pieces: aligned whatever dim is
   a.slices = p.slices;
+  a.reach = p.reach;
   a.accumulate = accumulate;
   a.once = streamed(n * dim * static_cast<int64_t>(sizeof(T)));
   // one more unit where a row may begin inside one

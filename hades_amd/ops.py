@@ -864,23 +864,23 @@ def _row_type(t, name):
 
 
 def _enter(t, name):
-    """(device, its current stream) of a call whose first tensor is t."""
-    if not t.is_cuda:
+    """(device number, its current stream) of a call whose first tensor is t."""
+    dev = t.get_device()
+    if dev < 0:
         raise RuntimeError("%s must be a device tensor" % name)
-    dev = t.device
-    if dev.index != _device_of_thread():
+    if dev != _device_of_thread():
         raise RuntimeError("%s is on %s, which is not the current device: launches go to the current device's "
-                           "stream" % (name, dev))
-    return dev, _raw_stream(dev.index)
+                           "stream" % (name, t.device))
+    return dev, _raw_stream(dev)
 
 
 def _row_stride(t, name, device):
-    """Elements between the rows of t (its last dimension), which lies on `device`."""
-    if t.device != device:
-        raise RuntimeError("%s must be a device tensor on %s" % (name, device))
-    if t.dim() == 0:
+    """Elements between the rows of t (its last dimension), which lies on device number `device`."""
+    if t.get_device() != device:
+        raise RuntimeError("%s must be a device tensor on cuda:%d" % (name, device))
+    if not t.shape:
         raise RuntimeError("%s must have at least one dimension" % name)
-    cols = t.size(-1)
+    cols = t.shape[-1]
     if t.is_contiguous() or t.numel() == 0:
         return cols
     try:
@@ -896,8 +896,8 @@ def _ids_type(ids, device):
     code = _ID_TYPES.get(ids.dtype)
     if code is None:
         raise RuntimeError("ID can only be int32 or int64 (ids is %s)" % ids.dtype)
-    if ids.device != device or not ids.is_contiguous():
-        raise RuntimeError("ids must be a contiguous tensor on %s" % device)
+    if ids.get_device() != device or not ids.is_contiguous():
+        raise RuntimeError("ids must be a contiguous tensor on cuda:%d" % device)
     return code
 
 
@@ -909,21 +909,24 @@ def _drop_args(dropout, device):
     if dropout is None:
         return _NO_DROP
     p, seed, offset = dropout
-    _check(0.0 <= p <= 1.0, "dropout: p must lie in [0, 1]")
+    if not 0.0 <= p <= 1.0:
+        raise RuntimeError("dropout: p must lie in [0, 1]")
     ptr = None
     if isinstance(offset, torch.Tensor):
-        _check(offset.dtype == torch.int64 and offset.numel() == 1 and offset.device == device,
+        _check(offset.dtype == torch.int64 and offset.numel() == 1 and offset.get_device() == device,
                "dropout: offset must be an int or an int64 tensor of one element on the device")
         ptr, offset = offset.data_ptr(), 0
-    _check(-(1 << 63) <= seed <= _U64 and 0 <= offset < (1 << 63),
-           "dropout: seed must fit 64 bits, offset must be in [0, 2^63)")
-    return float(p), seed & _U64, offset, ptr
+    if not (-(1 << 63) <= seed <= _U64 and 0 <= offset < (1 << 63)):
+        raise RuntimeError("dropout: seed must fit 64 bits, offset must be in [0, 2^63)")
+    return float(p), int(seed) & _U64, int(offset), ptr
 
 
 def _out_like(x, dtype, out, name="out"):
     """A dense tensor of x's shape and of dtype: `out` after its checks, or a new one."""
     if out is None:
-        return torch.empty_like(x) if x.dtype == dtype and x.is_contiguous() else x.new_empty(x.shape, dtype=dtype)
+        if x.dtype == dtype:
+            return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+        return x.new_empty(x.shape, dtype=dtype)
     _check(out.device == x.device and out.is_contiguous(), "%s must be a contiguous tensor on %s" % (name, x.device))
     _check(out.shape == x.shape and out.dtype == dtype, "%s has the wrong shape/dtype" % name)
     return out
@@ -938,7 +941,8 @@ def embed(weight, ids, scale=1.0, dropout=None, out=None):
     ids.shape + (dim,).  weight [num_rows, dim] may be a row-strided view; ids int32 or int64.  An
     id outside [0, num_rows) (padding, e.g. -1) gives a row of zeros."""
     dev, stream = _enter(weight, "weight")
-    _check(weight.dim() == 2 and weight.size(1) >= 1, "weight must be [num_rows, dim]")
+    if weight.dim() != 2 or weight.shape[1] < 1:
+        raise RuntimeError("weight must be [num_rows, dim]")
     dtype, stride = _row_type(weight, "weight"), _row_stride(weight, "weight", dev)
     itype = _ids_type(ids, dev)
     drop = _drop_args(dropout, dev)
@@ -947,10 +951,10 @@ def embed(weight, ids, scale=1.0, dropout=None, out=None):
     if out is None:
         out = weight.new_empty(shape)
     else:
-        _check(out.device == dev and out.is_contiguous(), "out must be a contiguous tensor on %s" % dev)
+        _check(out.get_device() == dev and out.is_contiguous(), "out must be a contiguous tensor on cuda:%d" % dev)
         _check(out.shape == shape and out.dtype == weight.dtype, "out has the wrong shape/dtype")
     _lib.call("hades_embed", weight.data_ptr(), stride, num_rows, ids.data_ptr(), ids.numel(), out.data_ptr(), dim,
-              dtype, itype, scale, *drop, stream)
+              dtype, itype, float(scale), *drop, stream)
     return out
 
 
@@ -963,11 +967,12 @@ def embed_grad(grad, ids, num_rows, scale=1.0, padding_idx=None, dropout=None, o
     ([num_rows, dim], may be row-strided) has grad's type or float32, as has `out_dtype`."""
     dev, stream = _enter(grad, "grad")
     dtype, stride = _row_type(grad, "grad"), _row_stride(grad, "grad", dev)
-    dim, n = grad.size(-1), ids.numel()
+    dim, n = grad.shape[-1], ids.numel()
     itype = _ids_type(ids, dev)
-    _check(dim >= 1 and grad.numel() == n * dim, "grad must have one row per id")
-    _check(num_rows >= 0, "num_rows must be >= 0")
-    _check(padding_idx is None or 0 <= padding_idx < num_rows, "padding_idx must be in [0, num_rows)")
+    if dim < 1 or grad.numel() != n * dim:
+        raise RuntimeError("grad must have one row per id")
+    if num_rows < 0 or not (padding_idx is None or 0 <= padding_idx < num_rows):
+        raise RuntimeError("num_rows must be >= 0 and padding_idx in [0, num_rows)")
     drop = _drop_args(dropout, dev)
     if out is None:
         _check(not accumulate, "accumulate needs out")
@@ -978,7 +983,7 @@ def embed_grad(grad, ids, num_rows, scale=1.0, padding_idx=None, dropout=None, o
     ws = grad.new_empty(nbytes, dtype=torch.uint8)
     _lib.call("hades_embed_grad", grad.data_ptr(), stride, ids.data_ptr(), n, out.data_ptr(),
               _row_stride(out, "out", dev), num_rows, dim, dtype, _ROW_TYPES[out.dtype], itype,
-              -1 if padding_idx is None else padding_idx, bool(accumulate), scale, *drop, ws.data_ptr(), nbytes, stream)
+              -1 if padding_idx is None else int(padding_idx), bool(accumulate), float(scale), *drop, ws.data_ptr(), nbytes, stream)
     return out
 
 
@@ -1009,23 +1014,25 @@ def dropout_grad(grad, p, seed, offset, out=None):
 
 def _weight_type(weight, x, cols, name):
     """C type of a norm's weight beside rows x"""
-    if (weight.device != x.device or weight.dim() != 1 or weight.size(0) != cols or not weight.is_contiguous()
-            or (weight.dtype != x.dtype and weight.dtype != torch.float32)):
+    code = _ROW_TYPES.get(weight.dtype)
+    if (weight.get_device() != x.get_device() or weight.shape != (cols,) or not weight.is_contiguous()
+            or (weight.dtype != x.dtype and code != _lib.F32)):
         raise RuntimeError("weight must be contiguous [columns of %s] on %s, of %s's dtype or float32"
                            % (name, x.device, name))
-    return _ROW_TYPES[weight.dtype]
+    return code
 
 
 def _norm_args(x, weight, residual, dropout, dev, h_out):
     """(type, row stride, columns, residual's stride, weight's type, dropout, h) of a norm's forward call"""
     dtype, stride = _row_type(x, "x"), _row_stride(x, "x", dev)
     cols = x.size(-1)
-    _check(cols >= 1, "x must have rows of at least one value")
+    if cols < 1:
+        raise RuntimeError("x must have rows of at least one value")
     h_dtype, res_stride, weight_type = x.dtype, 0, dtype
     if residual is not None:
         h_dtype = residual.dtype
-        _check(residual.shape == x.shape and (h_dtype == x.dtype or h_dtype == torch.float32),
-               "residual must have x's shape, and x's dtype or float32")
+        if residual.shape != x.shape or (h_dtype != x.dtype and h_dtype != torch.float32):
+            raise RuntimeError("residual must have x's shape, and x's dtype or float32")
         res_stride = _row_stride(residual, "residual", dev)
     if weight is not None:
         weight_type = _weight_type(weight, x, cols, "x")
@@ -1047,7 +1054,7 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, dropout=None, out=None, h_
     rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
     _lib.call("hades_rms_norm", x.data_ptr(), stride, _ptr_or_none(residual), res_stride, _ptr_or_none(weight),
               y.data_ptr(), None, None if h is x else h.data_ptr(), rstd.data_ptr(), rstd.numel(), cols, dtype,
-              _ROW_TYPES[h.dtype], weight_type, 0, eps, *drop, stream)
+              _ROW_TYPES[h.dtype], weight_type, 0, float(eps), *drop, stream)
     return y, h, rstd
 
 
@@ -1065,7 +1072,7 @@ def rms_norm_8bit(x, weight=None, eps=1e-6, residual=None, group=0, dropout=None
     scales = x.new_empty((*x.shape[:-1], groups), dtype=torch.float32)
     _lib.call("hades_rms_norm", x.data_ptr(), stride, _ptr_or_none(residual), res_stride, _ptr_or_none(weight),
               q.data_ptr(), scales.data_ptr(), None if h is x else h.data_ptr(), None, scales.numel() // groups, cols,
-              dtype, _ROW_TYPES[h.dtype], weight_type, group, eps, *drop, stream)
+              dtype, _ROW_TYPES[h.dtype], weight_type, int(group), float(eps), *drop, stream)
     return q, scales, h
 
 
@@ -1077,21 +1084,24 @@ def rms_norm_grad(grad, h, weight, rstd, grad_h=None, dropout=None, weight_grad=
     grad_residual None without residual_grad."""
     dev, stream = _enter(grad, "grad")
     dtype, grad_stride = _row_type(grad, "grad"), _row_stride(grad, "grad", dev)
-    cols = grad.size(-1)
-    _check(cols >= 1, "grad must have rows of at least one value")
-    _check(h.shape == grad.shape and (h.dtype == grad.dtype or h.dtype == torch.float32),
-           "h must have grad's shape, and grad's dtype or float32")
-    _check(grad_h is None or (grad_h.shape == h.shape and grad_h.dtype == h.dtype),
-           "grad_h must have h's shape and dtype")
-    _check(rstd.device == dev and rstd.dtype == torch.float32 and rstd.is_contiguous()
-           and rstd.shape == grad.shape[:-1], "rstd must be the contiguous float32 tensor that rms_norm returned")
+    shape, h_dtype = grad.shape, h.dtype
+    cols = shape[-1]
+    if cols < 1:
+        raise RuntimeError("grad must have rows of at least one value")
+    if h.shape != shape or (h_dtype != grad.dtype and h_dtype != torch.float32):
+        raise RuntimeError("h must have grad's shape, and grad's dtype or float32")
+    if grad_h is not None and (grad_h.shape != shape or grad_h.dtype != h_dtype):
+        raise RuntimeError("grad_h must have h's shape and dtype")
+    if (rstd.get_device() != dev or rstd.dtype != torch.float32 or not rstd.is_contiguous()
+            or rstd.shape != shape[:-1]):
+        raise RuntimeError("rstd must be the contiguous float32 tensor that rms_norm returned")
     weight_type = dtype if weight is None else _weight_type(weight, grad, cols, "grad")
     drop = _drop_args(dropout, dev)
     h_stride = _row_stride(h, "h", dev)
     gh_stride = 0 if grad_h is None else _row_stride(grad_h, "grad_h", dev)
     grad_x = _out_like(grad, grad.dtype, None)
-    apart = residual_grad and (dropout is not None or h.dtype != grad.dtype)
-    grad_res = _out_like(grad, h.dtype, None) if apart else None
+    apart = residual_grad and (dropout is not None or h_dtype != grad.dtype)
+    grad_res = _out_like(grad, h_dtype, None) if apart else None
     rows, nbytes = rstd.numel(), 0
     grad_w = ws = None
     if weight is not None and weight_grad:
@@ -1100,6 +1110,6 @@ def rms_norm_grad(grad, h, weight, rstd, grad_h=None, dropout=None, weight_grad=
         ws = grad.new_empty(nbytes, dtype=torch.uint8)
     _lib.call("hades_rms_norm_grad", grad.data_ptr(), grad_stride, h.data_ptr(), h_stride, _ptr_or_none(weight),
               rstd.data_ptr(), _ptr_or_none(grad_h), gh_stride, grad_x.data_ptr(), _ptr_or_none(grad_res),
-              _ptr_or_none(grad_w), rows, cols, dtype, _ROW_TYPES[h.dtype], weight_type, *drop, _ptr_or_none(ws),
+              _ptr_or_none(grad_w), rows, cols, dtype, _ROW_TYPES[h_dtype], weight_type, *drop, _ptr_or_none(ws),
               nbytes, stream)
     return grad_x, (grad_res if apart else grad_x) if residual_grad else None, grad_w
