@@ -130,11 +130,15 @@ struct DropKeys {
       k0 += 0x9E3779B9u;
       k1 += 0xBB67AE85u;
     }
+    // both halves of a word without taking it apart: the upper one reaches the threshold if the word is
+    // above threshold * 65536 - 1 (2^32 - 1 for p = 1, where nothing is kept)
     const uint32_t w[4] = {c0, c1, c2, c3};
+    const uint16_t low = static_cast<uint16_t>(threshold - 1u);
+    const uint32_t high = (threshold << 16) - 1u;
 #pragma unroll
-    for (int j = 0; j < kPiece; ++j) {
-      const uint32_t bits = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu;
-      v[j] = bits >= threshold ? v[j] * factor : 0.0f;
+    for (int j = 0; j < kPiece; j += 2) {
+      v[j] = static_cast<uint16_t>(w[j >> 1]) > low ? v[j] * factor : 0.0f;
+      v[j + 1] = w[j >> 1] > high ? v[j + 1] * factor : 0.0f;
     }
     return v;
   }
