@@ -18,7 +18,7 @@ namespace hades {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kE4m3Max = 448.0f;
+constexpr float kPerE4m3Max = 1.0f / 448.0f;   // of e4m3's largest value
 constexpr int64_t kMaxPieces = 2048;   // of a row that stays in registers
 constexpr int64_t kMostThreads = int64_t(1) << 32;   // of a launch
 constexpr int64_t kCus = 256;
@@ -29,11 +29,61 @@ constexpr int64_t kGradOne = 768;
 
 constexpr int kMaxWaves = 16;   // of a block
 
-// a weight, whose type is the rows' T or float32
+// A weight's piece, whose type is the rows' T or float32, as it lies in memory: nothing waits for it until it
+// is used.
+struct WeightPiece {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  typedef u32x4 u32x4u __attribute__((aligned(2)));
+  u32x4 lo, hi;
+
+  template <typename T>
+  __device__ __forceinline__ void load(const void* p, int64_t piece, bool f32, int valid) {
+    if (f32 || sizeof(T) == 4) {
+      const float* const q = static_cast<const float*>(p) + piece * kPiece;
+      if (valid >= kPiece) {
+        lo = *reinterpret_cast<const u32x4u*>(q);
+        hi = *reinterpret_cast<const u32x4u*>(q + 4);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          lo[j] = j < valid ? __float_as_uint(q[j]) : 0u;
+          hi[j] = j + 4 < valid ? __float_as_uint(q[j + 4]) : 0u;
+        }
+      }
+    } else {
+      const uint16_t* const q = static_cast<const uint16_t*>(p) + piece * kPiece;
+      if (valid >= kPiece) {
+        lo = *reinterpret_cast<const u32x4u*>(q);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          lo[j] = (2 * j < valid ? uint32_t(q[2 * j]) : 0u) | (2 * j + 1 < valid ? uint32_t(q[2 * j + 1]) << 16 : 0u);
+      }
+    }
+  }
+
+  template <typename T>
+  __device__ __forceinline__ f32x8 value(bool f32) const {
+    f32x8 r;
+    if (f32 || sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        r[j] = __uint_as_float(lo[j]);
+        r[j + 4] = __uint_as_float(hi[j]);
+      }
+      return r;
+    }
+    typename Vec8<T>::V v;
+    __builtin_memcpy(&v, &lo, 16);   // (unused where T is float32)
+    return __builtin_convertvector(v, f32x8);
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ f32x8 load_weight(const void* p, int64_t piece, bool f32, int valid) {
-  return f32 ? load8(static_cast<const float*>(p) + piece * kPiece, valid)
-             : load8(static_cast<const T*>(p) + piece * kPiece, valid);
+  WeightPiece w;
+  w.template load<T>(p, piece, f32, valid);
+  return w.template value<T>(f32);
 }
 
 // a * b summed
@@ -51,8 +101,7 @@ __device__ __forceinline__ float dot8(f32x8 a, f32x8 b) {
 // call; `shared` has kMaxWaves values then.
 template <int T>
 __device__ __forceinline__ float row_sum(float v, float* shared) {
-#pragma unroll
-  for (int d = 1; d < (T ? T : kWave); d <<= 1) v += __shfl_xor(v, d, kWave);
+  v = lanes_sum<T ? T : kWave>(v);
   if (T == 0) {
     const int waves = blockDim.x / kWave;
     __syncthreads();   // `shared` may still be read for the value before
@@ -64,17 +113,8 @@ __device__ __forceinline__ float row_sum(float v, float* shared) {
   return v;
 }
 
-// Largest magnitude over groups of `lanes` lanes of a wave (a power of two), as bits: magnitudes
-// compare like whole numbers, and a NaN counts as larger than an infinity.
-__device__ __forceinline__ uint32_t lanes_max(uint32_t v, int lanes) {
-  for (int d = 1; d < lanes; d <<= 1) {
-    const uint32_t o = __shfl_xor(v, d, kWave);
-    v = o > v ? o : v;
-  }
-  return v;
-}
-
-// (a NaN among them is the largest here too)
+// The largest magnitude as bits: magnitudes compare like whole numbers, and a NaN counts as larger than an
+// infinity.
 __device__ __forceinline__ uint32_t max8(f32x8 v) {
   float m = fabsf(v[0]);
 #pragma unroll
@@ -84,13 +124,13 @@ __device__ __forceinline__ uint32_t max8(f32x8 v) {
 
 // Eight values in units of `scale`, rounded to e4m3 (nearest even).  scale is the largest magnitude of
 // the group over 448, so a value in its units is at most 448 (1 + 2^-22), which rounds to 448, the type's
-// largest.  One division a piece, its reciprocal times each value: a value next to a tie may fall to the
-// other side of it than the quotient would, 2^-23 of it away.  Where the reciprocal would overflow, or scale is
+// largest.  Each value is multiplied by one reciprocal (to 2^-23): a value next to a tie may fall to the other
+// side of it than the quotient would.  Where the reciprocal would overflow, or scale is
 // subnormal and coarse, every value is divided; a group of zeros (scale 0) gives zeros.
 __device__ __forceinline__ void store_e4m3(uint8_t* __restrict__ p, f32x8 v, float scale, int valid) {
   f32x8 u;
   if (scale >= 0x1p-120f) {
-    u = v * (1.0f / scale);
+    u = v * __builtin_amdgcn_rcpf(scale);
   } else {
 #pragma unroll
     for (int j = 0; j < kPiece; ++j) u[j] = scale > 0.0f ? v[j] / scale : 0.0f;
@@ -125,7 +165,7 @@ struct NormArgs {
   int weight_f32;
   int group_lanes;        // lanes that share a scale; 0: the row
   int64_t groups;         // scales of a row
-  float eps;
+  float eps, inv_cols;
   DropArgs drop;
 };
 
@@ -136,11 +176,14 @@ __device__ __forceinline__ int valid_of(int64_t cols, int64_t piece) {
 
 template <typename X, typename S>
 __device__ __forceinline__ f32x8 load_h(const NormArgs& a, const DropKeys& keys, int64_t row, int64_t piece, int valid) {
-  f32x8 v = load8(static_cast<const X*>(a.x) + row * a.x_stride + piece * kPiece, valid);
-  f32x8 r;
-  if (a.residual != nullptr) r = load8(static_cast<const S*>(a.residual) + row * a.res_stride + piece * kPiece, valid);
+  // (raw, so that nothing waits for x before the residual's load is under way)
+  const typename Vec8<X>::V raw = load8_raw(static_cast<const X*>(a.x) + row * a.x_stride + piece * kPiece, valid);
+  typename Vec8<S>::V res;
+  if (a.residual != nullptr)
+    res = load8_raw(static_cast<const S*>(a.residual) + row * a.res_stride + piece * kPiece, valid);
+  f32x8 v = __builtin_convertvector(raw, f32x8);
   if (keys.on()) v = keys.apply(v, static_cast<uint32_t>(row), static_cast<uint32_t>(piece));
-  if (a.residual != nullptr) v += r;
+  if (a.residual != nullptr) v += __builtin_convertvector(res, f32x8);
   return v;
 }
 
@@ -150,19 +193,20 @@ __global__ __launch_bounds__(T ? kThreads : kMaxWaves* kWave) void rms_norm_kern
   __shared__ float shared[kMaxWaves];
   const DropKeys keys(a.drop);
   const int lanes = T ? T : blockDim.x;
-  const int lane = T ? threadIdx.x % T : threadIdx.x;
+  const int lane = T ? threadIdx.x % (T ? T : 1) : threadIdx.x;
   const int64_t row = T ? static_cast<int64_t>(blockIdx.x) * (kThreads / (T ? T : 1)) + threadIdx.x / (T ? T : 1)
                         : static_cast<int64_t>(blockIdx.x);
   const bool in = row < a.rows;
-  f32x8 h[K], w[K];
+  f32x8 h[K];
+  WeightPiece w[K];
   int valid[K];
   float ss = 0.0f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int64_t piece = k * lanes + lane;
     valid[k] = in ? valid_of(a.cols, piece) : 0;
+    if (a.weight != nullptr) w[k].template load<X>(a.weight, piece, a.weight_f32, valid[k]);
     h[k] = load_h<X, S>(a, keys, row, piece, valid[k]);
-    if (a.weight != nullptr) w[k] = load_weight<X>(a.weight, piece, a.weight_f32, valid[k]);
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -170,13 +214,13 @@ __global__ __launch_bounds__(T ? kThreads : kMaxWaves* kWave) void rms_norm_kern
     ss += dot8(h[k], h[k]);
   }
   ss = row_sum<T>(ss, shared);
-  const float rstd = 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps);
+  const float rstd = rsqrtf(fmaf(ss, a.inv_cols, a.eps));
   if (a.rstd != nullptr && lane == 0 && in) a.rstd[row] = rstd;
   uint32_t top = 0;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     h[k] *= rstd;
-    if (a.weight != nullptr) h[k] *= w[k];
+    if (a.weight != nullptr) h[k] *= w[k].template value<X>(a.weight_f32);
     if (!kEight) {
       store8(static_cast<X*>(a.y) + row * a.cols + (k * lanes + lane) * kPiece, h[k], valid[k]);
     } else if (a.group_lanes == 0) {
@@ -200,7 +244,7 @@ __global__ __launch_bounds__(T ? kThreads : kMaxWaves* kWave) void rms_norm_kern
     const int piece = k * lanes + lane;
     uint32_t m = top;
     if (a.group_lanes != 0) m = lanes_max(max8(h[k]), T && a.group_lanes > T ? T : a.group_lanes);
-    const float scale = __uint_as_float(m) / kE4m3Max;
+    const float scale = __uint_as_float(m) * kPerE4m3Max;
     const bool first = a.group_lanes == 0 ? piece == 0 : (piece & (a.group_lanes - 1)) == 0;
     if (first && valid[k] > 0) a.scales[row * a.groups + (a.group_lanes == 0 ? 0 : piece / a.group_lanes)] = scale;
     store_e4m3(static_cast<uint8_t*>(a.y) + row * a.cols + static_cast<int64_t>(piece) * kPiece, h[k], scale, valid[k]);
@@ -224,7 +268,7 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs a) {
     ss += dot8(h, h);
   }
   ss = row_sum<0>(ss, shared);
-  const float rstd = 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps);
+  const float rstd = rsqrtf(fmaf(ss, a.inv_cols, a.eps));
   if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = rstd;
   uint32_t top = 0;
   if (kEight && a.group_lanes == 0) {
@@ -254,7 +298,7 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs a) {
       continue;
     }
     const uint32_t m = a.group_lanes != 0 ? lanes_max(max8(y), a.group_lanes) : top;
-    const float scale = __uint_as_float(m) / kE4m3Max;
+    const float scale = __uint_as_float(m) * kPerE4m3Max;
     const bool first = a.group_lanes == 0 ? piece == 0 : (piece & (a.group_lanes - 1)) == 0;
     if (first && valid > 0) a.scales[row * a.groups + (a.group_lanes == 0 ? 0 : piece / a.group_lanes)] = scale;
     store_e4m3(static_cast<uint8_t*>(a.y) + at, y, scale, valid);
@@ -285,7 +329,7 @@ __global__ __launch_bounds__(T ? kThreads : kMaxWaves* kWave, T == 0 && K == 1 ?
   __shared__ f32x8 parts[kRows > 1 ? kThreads * K : 1];
   const DropKeys keys(a.drop);
   const int lanes = T ? T : blockDim.x;
-  const int lane = T ? threadIdx.x % T : threadIdx.x;
+  const int lane = T ? threadIdx.x % (T ? T : 1) : threadIdx.x;
   const int sub = T ? threadIdx.x / (T ? T : 1) : 0;
   const float inv_cols = 1.0f / static_cast<float>(a.cols);
   const f32x8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -450,20 +494,27 @@ int64_t grad_threads(int64_t pieces) {
   return ceil_div(ceil_div(pieces, pieces <= kGradOne ? 1 : 2), kWave) * kWave;
 }
 
-// Blocks of the gradient kernel = rows of grad_weight's partial sum: as many as are resident at once, six
-// waves on each SIMD (80 registers) for 16-bit rows.  float32 rows have twice the bytes in flight: 16 waves a
-// compute unit do for them, and fewer partial rows are written (rows of 1 024: 139 us, with 24 waves 145).
-// The forms with 94 and 128 registers have five and four waves.
+// Blocks of the gradient kernel = rows of grad_weight's partial sum.  More waves on a compute unit than it
+// takes to keep memory busy cost time: 12 for 16-bit rows, 8 for float32 rows, which have twice the bytes in
+// flight, but two blocks where they fit (one of them waits for its row's sum meanwhile).  16-bit rows that leave
+// lanes idle want as many as are resident.  us for 2^26 bfloat16 values with dropout, 12 / 24 waves: rows of 1 024
+// 131 / 146, 2 048 132 / 141, 768 203 / 147, 1 000 173 / 150; 2^25 float32 values, 8 / 16 waves: 2 048 127 / 135.
 int64_t grad_blocks(int64_t rows, int64_t cols, bool f32) {
   const int64_t pieces = ceil_div(cols, kPiece);
   if (pieces > kMaxPieces) return rows < 64 ? rows : 64;
   int64_t lanes = 8;
   while (lanes < kWave && lanes < pieces) lanes *= 2;
   const int64_t blocks = pieces <= kWave ? ceil_div(rows, kThreads / lanes) : rows;
-  const int64_t waves = pieces <= kWave ? 20 : (pieces <= kGradOne && !f32 ? 24 : 16);
-  int64_t per_cu = waves / (grad_threads(pieces) / kWave);
-  if (per_cu < 1) per_cu = 1;
+  const int64_t block = grad_threads(pieces) / kWave;
+  const bool full = pieces <= kWave ? pieces == lanes : pieces % kWave == 0;
+  int64_t per_cu = (f32 ? 8 : (full ? 12 : (pieces <= kWave ? 20 : 24))) / block;
+  if (per_cu < 2) per_cu = pieces <= kGradOne || block <= 8 ? 2 : 1;
   return blocks < per_cu * kCus ? blocks : per_cu * kCus;
+}
+
+size_t grad_bytes(int64_t rows, int64_t cols, bool f32) {
+  const size_t b = static_cast<size_t>(grad_blocks(rows > 0 ? rows : 1, cols, f32)) * cols * sizeof(float);
+  return (b + 255) & ~size_t(255);
 }
 
 template <typename X, typename S>
@@ -534,6 +585,7 @@ int hades_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_
   a.group_lanes = static_cast<int>(group / kPiece);
   a.groups = group == 0 ? 1 : ceil_div(cols, group);
   a.eps = eps;
+  a.inv_cols = static_cast<float>(1.0 / static_cast<double>(cols));
   a.drop = drop;
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define HADES_NORM_TYPE(X_, S_) \
@@ -550,8 +602,8 @@ int hades_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_
 
 size_t hades_rms_norm_grad_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows < 0 || cols < 1) return 0;
-  const size_t b = static_cast<size_t>(grad_blocks(rows > 0 ? rows : 1, cols, false)) * cols * sizeof(float);
-  return (b + 255) & ~size_t(255);
+  const size_t narrow = grad_bytes(rows, cols, false), wide = grad_bytes(rows, cols, true);
+  return narrow > wide ? narrow : wide;   // of either type of rows
 }
 
 int hades_rms_norm_grad(const void* grad, int64_t grad_stride, const void* h, int64_t h_stride, const void* weight,
@@ -572,7 +624,7 @@ int hades_rms_norm_grad(const void* grad, int64_t grad_stride, const void* h, in
   HADES_REQUIRE(grad_stride >= cols || rows <= 1, "row stride below cols");
   HADES_REQUIRE(h_stride >= cols || rows <= 1, "row stride below cols");
   HADES_REQUIRE(!grad_h || grad_h_stride >= cols || rows <= 1, "row stride below cols");
-  const size_t need = hades_rms_norm_grad_workspace_bytes(rows, cols);
+  const size_t need = grad_bytes(rows, cols, dtype == HADES_F32);
   if (grad_weight && (workspace == nullptr || workspace_bytes < need))
     return set_error(HADES_ERR_WORKSPACE, "rms_norm_grad workspace too small: need %zu bytes, got %zu", need,
                      workspace_bytes);

@@ -100,6 +100,52 @@ __device__ __forceinline__ void store8(T* __restrict__ p, f32x8 v, int valid) {
     if (j < valid) p[j] = static_cast<T>(v[j]);
 }
 
+// The value of lanes that mirror one another, from pairs up to the halves of the wave: after the steps below `n`
+// every group of n lanes has combined all its values, whatever the order of the lanes is in a step.
+template <int kStep>
+__device__ __forceinline__ uint32_t partner(uint32_t v) {
+  if (kStep == 1) return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);    // lanes 1 0 3 2
+  if (kStep == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);    // lanes 2 3 0 1
+  if (kStep == 4) return __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);   // eight lanes reversed
+  return __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true);                   // sixteen lanes reversed
+}
+
+// Sum over each group of N lanes of a full wave (N a power of two); every lane gets its group's.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if (N > 1) v += __uint_as_float(partner<1>(__float_as_uint(v)));
+  if (N > 2) v += __uint_as_float(partner<2>(__float_as_uint(v)));
+  if (N > 4) v += __uint_as_float(partner<4>(__float_as_uint(v)));
+  if (N > 8) v += __uint_as_float(partner<8>(__float_as_uint(v)));
+  if (N > 16) {   // rows of 16 lanes: the two results hold the even rows' and the odd rows' values
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (N > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+
+// The largest of each group of n lanes (n a power of two, the same for the whole wave)
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v, int n) {
+  const auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  if (n > 1) v = larger(v, partner<1>(v));
+  if (n > 2) v = larger(v, partner<2>(v));
+  if (n > 4) v = larger(v, partner<4>(v));
+  if (n > 8) v = larger(v, partner<8>(v));
+  if (n > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = larger(r[0], r[1]);
+  }
+  if (n > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = larger(r[0], r[1]);
+  }
+  return v;
+}
+
 // Philox4x32 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", 2011) with
 // seven rounds, the fewest that pass the paper's statistical tests: 128 bits for eight values of a row.
 // Per piece 14 products of 32 x 32 bits; a dropout of bfloat16 rows stays bound by memory.

@@ -139,3 +139,20 @@ def test_host_tensors_are_refused():
                  lambda: ops.rms_norm_grad(x, x, None, x[:, 0])):
         with pytest.raises(RuntimeError, match="device tensor"):
             call()
+
+
+def test_rms_norm_grad_workspace_query_covers_every_type():
+    """The bytes that the query names are enough for rows of any type, whichever needs more of them (checked
+    before any launch: the workspace's alignment is looked at after its size, and is wrong here)."""
+    lib = _lib.load()
+    for cols in (1, 8, 64, 65, 100, 512, 513, 768, 1000, 1024, 2048, 4096, 6144, 6145, 8192, 16384, 16385):
+        for rows in (1, 5, 511, 512, 513, 3000, 5000, 1_000_000):
+            nbytes = _lib.query("hades_rms_norm_grad_workspace_bytes", rows, cols)
+            short = set()
+            for dtype in (_lib.F32, _lib.F16, _lib.BF16):
+                def call(size):
+                    return lib.hades_rms_norm_grad(ONE, cols, ONE, cols, ONE, ONE, NULL, 0, ONE, NULL, ONE, rows, cols,
+                                                   dtype, dtype, dtype, *DROP, ctypes.c_void_p(8), size, NULL)
+                assert call(nbytes) == 1 and b"aligned" in lib.hades_last_error()
+                short.add(call(nbytes - 256))
+            assert 3 in short
