@@ -39,7 +39,7 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(DropoutArgs<T> a) {
   int64_t row[kPieces];
   uint32_t piece[kPieces];
   int valid[kPieces];
-  f32x8 v[kPieces], res[kPieces];
+  typename Vec8<T>::V v[kPieces], res[kPieces];   // as they lie in memory: nothing waits before all are under way
 #pragma unroll
   for (int k = 0; k < kPieces; ++k) {
     const uint32_t at = rest + threadIdx.x + k * kThreads;
@@ -50,13 +50,19 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(DropoutArgs<T> a) {
     const int64_t left = a.cols - static_cast<int64_t>(piece[k]) * kPiece;
     valid[k] = in ? (left < kPiece ? static_cast<int>(left) : kPiece) : 0;
     const int64_t col = static_cast<int64_t>(piece[k]) * kPiece;
-    v[k] = load8<T, kOnce>(a.x + row[k] * a.x_stride + col, valid[k]);
-    if (a.residual != nullptr) res[k] = load8<T, kOnce>(a.residual + row[k] * a.res_stride + col, valid[k]);
+    v[k] = load8_raw<T, kOnce>(a.x + row[k] * a.x_stride + col, valid[k]);
+  }
+  if (a.residual != nullptr) {
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k)
+      res[k] = load8_raw<T, kOnce>(a.residual + row[k] * a.res_stride + static_cast<int64_t>(piece[k]) * kPiece,
+                                   valid[k]);
   }
 #pragma unroll
   for (int k = 0; k < kPieces; ++k) {
-    f32x8 y = keys.on() ? keys.apply(v[k], static_cast<uint32_t>(row[k]), piece[k]) : v[k];
-    if (a.residual != nullptr) y += res[k];
+    f32x8 y = __builtin_convertvector(v[k], f32x8);
+    if (keys.on()) y = keys.apply(y, static_cast<uint32_t>(row[k]), piece[k]);
+    if (a.residual != nullptr) y += __builtin_convertvector(res[k], f32x8);
     store8(a.out + row[k] * a.cols + static_cast<int64_t>(piece[k]) * kPiece, y, valid[k]);
   }
 }
