@@ -128,7 +128,8 @@ class InputStage(nn.Module):
     y = h / sqrt(mean(h^2) + norm_eps) * weight.
 
     The masks of a module are drawn from (seed, offset); without an explicit offset every forward call in
-    training takes the next one (kept with the state dict).  A captured forward needs `offset`, an int64
+    training takes the next one (kept with the state dict).  Give the modules of one model, and the
+    processes of a data-parallel run, different seeds.  A captured forward needs `offset`, an int64
     tensor of one element on the device that the captured step counts up itself: replays of one number
     would drop the same values every time."""
 

@@ -846,14 +846,16 @@ def bucket_by_owner(ids, grad=None, cnt=None, partition_range=None, local_num_gp
 # stored: value (row, column) is a function of the three and of its row and column alone.  p counts in
 # 65536ths (to the nearest), seed is any 64-bit number, offset an int or an int64 tensor of one element
 # on the device, read when the kernel runs (a captured step that adds to it draws new masks on replay).
-# Two calls of one step need different offsets, or their masks are equal.
+# Two calls of one step need different offsets or seeds, or their masks are equal; so do the processes of
+# a data-parallel run.
 _ROW_TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _ID_TYPES = {torch.int32: _lib.I32, torch.int64: _lib.I64}
 _U64 = (1 << 64) - 1
 
 
-_device_of_thread = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# (absent from a torch without a GPU runtime, where no tensor gets as far as these)
+_device_of_thread = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _row_type(t, name):

@@ -250,6 +250,29 @@ def test_embed_grad_of_one_token(cuda_device, n):
     assert not ops.embed_grad(g, ids, 5, padding_idx=3).any()
 
 
+@pytest.mark.parametrize("vocab", [1, 255, 257, 40_000, 262_145, 600_000, 1 << 20, (1 << 20) + 1])
+@pytest.mark.parametrize("n", [1, 64, 65, 1023, 1024, 1025, 131_072, 131_073])
+def test_embed_grad_sorts_every_batch_in_order(cuda_device, n, vocab):
+    """All forms of the sort (one tile, tiles, radix; tables on both sides of their limits).  The columns' weights
+    1, k and k^2 of every position k (mod 61) are whole numbers whose sums float32 holds exactly for the
+    tokens that are looked at: each token has to get its own positions, no other's and none twice."""
+    ids = token_ids(n, vocab, 3, 0.1)
+    ids[0] = vocab - 1
+    k = torch.arange(n) % 61
+    g = torch.stack((torch.ones(n), k.float(), (k * k).float()), 1)
+    want = torch.zeros((vocab, 3), dtype=torch.float64).index_add_(0, ids[ids >= 0], g[ids >= 0].double())
+    assert float(want.max()) < 2 ** 24 * 16      # beyond 2^24 the sum's steps may round
+    got = ops.embed_grad(g.cuda(), ids.cuda(), vocab).double().cpu()
+    exact = want.max(1).values < 2 ** 24
+    assert torch.equal(got[exact], want[exact])
+    within(got, want, want * (n * U))
+    out = torch.full((vocab, 3), 0.5, device="cuda")
+    got = ops.embed_grad(g.cuda(), ids.int().cuda(), vocab, out=out, accumulate=True, padding_idx=vocab - 1).double().cpu()
+    want[vocab - 1] = 0
+    small = want.max(1).values < 2 ** 22
+    assert torch.equal(got[small], want[small] + 0.5)
+
+
 def test_embed_grad_of_no_tokens_and_strided_rows(cuda_device):
     g = rows_of((9, 4, 50), torch.bfloat16, 1).cuda()
     ids = token_ids(9, 6, 2).cuda()
@@ -541,6 +564,15 @@ def test_offsets_past_32_bits(cuda_device):
     part = ops.rms_norm_grad(y[vocab - 3:], h[vocab - 3:], None, rstd[vocab - 3:])
     assert torch.equal(gr[vocab - 3:], part[1])
     within(gx[vocab - 3:], gr[vocab - 3:].double().cpu() * f, gr[vocab - 3:].double().cpu().abs() * 2 ** -6 + 1e-30)
+
+
+def test_more_than_2_to_31_pieces(cuda_device):
+    """A dropout in place over 2^34 values and more: the flat list of pieces passes 31 bits."""
+    rows, cols = (1 << 21) + 3, 8192
+    x = torch.ones((rows, cols), dtype=torch.bfloat16, device="cuda")
+    assert ops.dropout(x, 0.5, 1, 2, out=x) is x
+    for at in (0, rows // 2, rows - 1):
+        assert torch.equal(x[at:at + 1].double().cpu(), factors(np.arange(at, at + 1), cols, (0.5, 1, 2)))
 
 
 def test_refusals_on_device_tensors(cuda_device):
