@@ -384,6 +384,28 @@ def test_rms_norm_8bit(cuda_device, dtype, rows, cols, group):
     within(gh, h, off + half_step(dtype) * (h.abs() + off))
 
 
+def test_rms_norm_forms_agree(cuda_device):
+    """One row without a row dimension, a copy of h without residual, and the 8-bit form with dropout."""
+    x, w = rows_of((300,), torch.bfloat16, 1).cuda(), rows_of((300,), torch.float32, 2).cuda()
+    y, h, rstd = ops.rms_norm(x, w)
+    y2, h2, rstd2 = ops.rms_norm(x.view(1, 300), w, h_out=torch.empty((1, 300), dtype=torch.bfloat16, device="cuda"))
+    assert rstd.shape == () and torch.equal(y, y2[0]) and torch.equal(h2[0], x) and torch.equal(rstd, rstd2[0])
+    gx, gr, gw = ops.rms_norm_grad(y, h, w, rstd)
+    gx2, _, gw2 = ops.rms_norm_grad(y2, h2, w, rstd2, residual_grad=False)
+    assert torch.equal(gx, gx2[0]) and torch.equal(gw, gw2)
+    q, scales, h = ops.rms_norm_8bit(x, w, group=64)
+    assert q.shape == (300,) and scales.shape == (5,) and h is x
+    x, res, drop = rows_of((40, 300), torch.bfloat16, 3).cuda(), rows_of((40, 300), torch.float32, 4).cuda(), (0.3, 4, 5)
+    y, h, _ = ops.rms_norm(x, w, residual=res, dropout=drop)
+    q, scales, h8 = ops.rms_norm_8bit(x, w, residual=res, dropout=drop)
+    assert torch.equal(h, h8)
+    # y is rounded to bfloat16, q to e4m3 in units of the scale; both from the same float32 value
+    bound = y.double().abs() * (2 ** -8 + 2 ** -4 + 2 ** -11) + 2.0 ** -10 * scales.double()
+    within(q.float().double() * scales.double(), y, bound)
+    y, h, _ = ops.rms_norm(x, w, dropout=drop)
+    assert torch.equal(h, ops.dropout(x, *drop))
+
+
 def test_rms_norm_8bit_of_zeros_and_infinities(cuda_device):
     x = rows_of((4, 256), torch.float32, 1)
     x[1] = 0
