@@ -35,6 +35,8 @@ constexpr int64_t kCus = 256;
 // block of the one-piece form fits a compute unit, and nothing hides its waits for the row's sum (2^26
 // bfloat16 values with dropout in rows of 7 168 / 8 192: one piece 156 / 148 us, two 134 / 132).
 constexpr int64_t kGradOne = 768;
+// Steps of rows that one block takes alone, without the second launch that adds the blocks' partial rows
+constexpr int64_t kGradAlone = 4;
 
 constexpr int kMaxWaves = 16;   // of a block
 
@@ -323,7 +325,8 @@ struct NormGradArgs {
   const void* grad_h;    // may be null; the stream's type
   void* grad_x;          // rows' type
   void* grad_res;        // may be null; the stream's type
-  float* partial;        // [blocks][cols] rows of grad_weight's sum; null without grad_weight
+  float* partial;        // [blocks][cols] rows of grad_weight's sum; null without grad_weight or with ...
+  void* grad_weight;     // ... the result itself, of a call with one block
   int64_t grad_stride, h_stride, grad_h_stride, rows, cols;
   int weight_f32;
   DropArgs drop;
@@ -383,7 +386,7 @@ __global__ __launch_bounds__(T ? kThreads : kMaxWaves* kWave, T == 0 && K == 1 ?
       store8(static_cast<X*>(a.grad_x) + row * a.cols + piece * kPiece, d, valid[k]);
     }
   }
-  if (a.partial == nullptr) return;
+  if (a.partial == nullptr && a.grad_weight == nullptr) return;
   if (kRows > 1) {   // the rows of a block, in order
 #pragma unroll
     for (int k = 0; k < K; ++k) parts[k * kThreads + threadIdx.x] = dw[k];
@@ -396,7 +399,10 @@ __global__ __launch_bounds__(T ? kThreads : kMaxWaves* kWave, T == 0 && K == 1 ?
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int64_t piece = k * lanes + lane;
-    store8(a.partial + blockIdx.x * a.cols + piece * kPiece, dw[k], valid_of(a.cols, piece));
+    const int valid = valid_of(a.cols, piece);
+    if (a.partial != nullptr) store8(a.partial + blockIdx.x * a.cols + piece * kPiece, dw[k], valid);
+    else if (a.weight_f32) store8(static_cast<float*>(a.grad_weight) + piece * kPiece, dw[k], valid);
+    else store8(static_cast<X*>(a.grad_weight) + piece * kPiece, dw[k], valid);
   }
 }
 
@@ -515,13 +521,16 @@ int64_t grad_blocks(int64_t rows, int64_t cols, bool f32) {
   while (lanes < kWave && lanes < pieces) lanes *= 2;
   const int64_t blocks = pieces <= kWave ? ceil_div(rows, kThreads / lanes) : rows;
   const int64_t block = grad_threads(pieces) / kWave;
+  if (blocks <= kGradAlone) return 1;
   const bool full = pieces <= kWave ? pieces == lanes : pieces % kWave == 0;
   int64_t per_cu = (f32 ? 8 : (full ? 12 : (pieces <= kWave ? 20 : 24))) / block;
   if (per_cu < 2) per_cu = pieces <= kGradOne || block <= 8 ? 2 : 1;
   return blocks < per_cu * kCus ? blocks : per_cu * kCus;
 }
 
+// bytes of the partial rows; a call with one block, or none, has none
 size_t grad_bytes(int64_t rows, int64_t cols, bool f32) {
+  if (grad_blocks(rows, cols, f32) <= 1 && ceil_div(cols, kPiece) <= kMaxPieces) return 0;
   const size_t b = static_cast<size_t>(grad_blocks(rows > 0 ? rows : 1, cols, f32)) * cols * sizeof(float);
   return (b + 255) & ~size_t(255);
 }
@@ -633,8 +642,8 @@ int hades_rms_norm_grad(const void* grad, int64_t grad_stride, const void* h, in
   HADES_REQUIRE(grad_stride >= cols || rows <= 1, "row stride below cols");
   HADES_REQUIRE(h_stride >= cols || rows <= 1, "row stride below cols");
   HADES_REQUIRE(!grad_h || grad_h_stride >= cols || rows <= 1, "row stride below cols");
-  const size_t need = grad_bytes(rows, cols, dtype == HADES_F32);
-  if (grad_weight && (workspace == nullptr || workspace_bytes < need))
+  const size_t need = grad_weight ? grad_bytes(rows, cols, dtype == HADES_F32) : 0;
+  if (need != 0 && (workspace == nullptr || workspace_bytes < need))
     return set_error(HADES_ERR_WORKSPACE, "rms_norm_grad workspace too small: need %zu bytes, got %zu", need,
                      workspace_bytes);
   HADES_REQUIRE((align_of_ptr(workspace) & 255) == 0, "workspace must be 256-byte aligned");
@@ -646,7 +655,8 @@ int hades_rms_norm_grad(const void* grad, int64_t grad_stride, const void* h, in
   a.grad_h = grad_h;
   a.grad_x = grad_x;
   a.grad_res = grad_res;
-  a.partial = grad_weight ? static_cast<float*>(workspace) : nullptr;
+  a.partial = need != 0 ? static_cast<float*>(workspace) : nullptr;
+  a.grad_weight = grad_weight;
   a.grad_stride = grad_stride;
   a.h_stride = h_stride;
   a.grad_h_stride = grad_h_stride;
@@ -662,7 +672,7 @@ int hades_rms_norm_grad(const void* grad, int64_t grad_stride, const void* h, in
       rc = stream_dtype == HADES_F16 ? launch_norm_grad<f16, f16>(a, st) : launch_norm_grad<f16, float>(a, st);
     else rc = stream_dtype == HADES_BF16 ? launch_norm_grad<bf16, bf16>(a, st) : launch_norm_grad<bf16, float>(a, st);
   }
-  if (rc != HADES_OK || !grad_weight) return rc;
+  if (rc != HADES_OK || !grad_weight || (rows > 0 && need == 0)) return rc;
   const int64_t blocks = rows > 0 ? grad_blocks(rows, cols, dtype == HADES_F32) : 0;
   const dim3 grid(static_cast<unsigned>(ceil_div(cols, kWave))), block(kFoldWaves * kWave);
 #define HADES_FOLD(W_) \

@@ -1109,7 +1109,8 @@ def rms_norm_grad(grad, h, weight, rstd, grad_h=None, dropout=None, weight_grad=
     if weight is not None and weight_grad:
         grad_w = torch.empty_like(weight)
         nbytes = _lib.query("hades_rms_norm_grad_workspace_bytes", rows, cols)
-        ws = grad.new_empty(nbytes, dtype=torch.uint8)
+        if nbytes:      # (a few rows are one block's work and need none)
+            ws = grad.new_empty(nbytes, dtype=torch.uint8)
     _lib.call("hades_rms_norm_grad", grad.data_ptr(), grad_stride, h.data_ptr(), h_stride, _ptr_or_none(weight),
               rstd.data_ptr(), _ptr_or_none(grad_h), gh_stride, grad_x.data_ptr(), _ptr_or_none(grad_res),
               _ptr_or_none(grad_w), rows, cols, dtype, _ROW_TYPES[h_dtype], weight_type, *drop, _ptr_or_none(ws),

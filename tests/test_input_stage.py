@@ -109,7 +109,7 @@ def test_rms_norm_refusals():
 
 
 def test_rms_norm_grad_refusals():
-    ok = [ONE, 64, ONE, 64, ONE, ONE, NULL, 0, ONE, NULL, ONE, 10, 64, _lib.BF16, _lib.BF16, _lib.BF16, *DROP,
+    ok = [ONE, 64, ONE, 64, ONE, ONE, NULL, 0, ONE, NULL, ONE, 1000, 64, _lib.BF16, _lib.BF16, _lib.BF16, *DROP,
           ONE, 1 << 40, NULL]
 
     def bad(at, value, match, code=1):
@@ -154,5 +154,7 @@ def test_rms_norm_grad_workspace_query_covers_every_type():
                     return lib.hades_rms_norm_grad(ONE, cols, ONE, cols, ONE, ONE, NULL, 0, ONE, NULL, ONE, rows, cols,
                                                    dtype, dtype, dtype, *DROP, ctypes.c_void_p(8), size, NULL)
                 assert call(nbytes) == 1 and b"aligned" in lib.hades_last_error()
-                short.add(call(nbytes - 256))
-            assert 3 in short
+                if nbytes:      # (a few rows need no workspace at all)
+                    short.add(call(nbytes - 256))
+            assert 3 in short or not nbytes
+            assert nbytes or rows < 1000
