@@ -14,7 +14,7 @@
 // held in float32 and their order is fixed by (n, dim) and the sorted tokens, so results are the same
 // from run to run.  Three parts:
 //   tokens  positions in token order (stable) and row_start[v] = first of token v: one kernel for up to
-//           1 024 ids, two for up to 131 072, beyond that and for tables of more than 2^20 rows the
+//           4 096 ids, two for up to 131 072, beyond that and for tables of more than 2^20 rows the
 //           library's radix sort.  Blocks of the same launches write zeros meanwhile.
 //   sum     chunks of 8, 16 or 32 sorted positions, whatever the tokens' frequencies: one lane
 //           group walks the rows of a chunk for its columns and writes every token that begins in the
@@ -329,7 +329,14 @@ __global__ __launch_bounds__(kTileIds) void token_bucket_kernel(const uint32_t* 
   }
 }
 
-// A batch of one tile without the first kernel: the block of a bucket looks at all ids itself.
+// A batch of a few ids a thread without the first kernel: the block of a bucket looks at all ids itself, a wave at
+// 64 * kSmallSteps of them one after another.  us of the whole gradient with this kernel / with two, bfloat16:
+// 1 500 x 128 into 32 000 rows 17.3 / 22.3, 3 000 x 512 into 32 000 19.7 / 24.4, 4 096 x 1 024 into 32 000
+// 22.7 / 27.6; with eight steps a wave 8 192 x 128 into 32 000 takes 24.8 / 25.4, 6 000 x 512 float32 into
+// 50 257 34.8 / 30.7.
+constexpr int kSmallSteps = 4;
+constexpr int64_t kSmallIds = int64_t(kTileIds) * kSmallSteps;
+
 template <typename I>
 __global__ __launch_bounds__(kTileIds) void token_small_kernel(const I* __restrict__ ids, int64_t n, int64_t num_rows,
                                                                int64_t padding, int shift, uint32_t* __restrict__ perm,
@@ -342,17 +349,38 @@ __global__ __launch_bounds__(kTileIds) void token_small_kernel(const I* __restri
   const uint32_t v0 = blockIdx.x << shift;
   const uint32_t rows = static_cast<uint32_t>(num_rows);
   const uint32_t mine = rows - v0 < static_cast<uint32_t>(range) ? rows - v0 : static_cast<uint32_t>(range);
+  const int lane = threadIdx.x & (kWave - 1);
   const int wave = threadIdx.x / kWave;
-  const int64_t id = threadIdx.x < n ? static_cast<int64_t>(ids[threadIdx.x]) : int64_t(-1);
-  const bool real = static_cast<uint64_t>(id) < static_cast<uint64_t>(num_rows) && id != padding;
-  const uint32_t at = static_cast<uint32_t>(id) - v0;
-  const bool in = real && at < mine;
+  // every wave takes as many steps, so that places by wave, step and lane keep the order of positions
+  const int steps = static_cast<int>((n + kTileIds - 1) / kTileIds);
+  const uint32_t from = wave * steps * kWave + lane;
+  int64_t id[kSmallSteps];
+#pragma unroll
+  for (int k = 0; k < kSmallSteps; ++k)
+    id[k] = k < steps && from + k * kWave < n ? static_cast<int64_t>(ids[from + k * kWave]) : int64_t(-1);
   for (int k = threadIdx.x; k < kTileWaves * range; k += kTileIds) counts[k] = 0;
+  uint32_t below = 0;
+  uint32_t at[kSmallSteps];
+  bool in[kSmallSteps];
+#pragma unroll
+  for (int k = 0; k < kSmallSteps; ++k) {
+    const bool real = static_cast<uint64_t>(id[k]) < static_cast<uint64_t>(num_rows) && id[k] != padding;
+    at[k] = static_cast<uint32_t>(id[k]) - v0;
+    in[k] = real && at[k] < mine;
+    if (!in[k]) at[k] = 0;
+    below += real && static_cast<uint32_t>(id[k]) < v0;
+  }
   uint32_t base;   // tokens below the range
-  block_exclusive_sum<uint32_t, kTileIds>(real && static_cast<uint32_t>(id) < v0 ? 1u : 0u, scan, &base);
-  const uint64_t peers = peers_of(in ? at : 0u, shift, __ballot(in));
-  const uint32_t rank = ballot_rank(peers);
-  if (in && rank == 0) counts[wave * range + at] = static_cast<uint32_t>(__popcll(peers));
+  block_exclusive_sum<uint32_t, kTileIds>(below, scan, &base);
+  volatile uint32_t* const own = counts + wave * range;   // lanes read what other lanes of the wave wrote
+  uint64_t peers[kSmallSteps];
+#pragma unroll
+  for (int k = 0; k < kSmallSteps; ++k) {
+    peers[k] = __ballot(in[k]);
+    if (peers[k] == 0) continue;   // (the same for the whole wave)
+    peers[k] = peers_of(at[k], shift, peers[k]);
+    if (in[k] && ballot_rank(peers[k]) == 0) own[at[k]] = own[at[k]] + static_cast<uint32_t>(__popcll(peers[k]));
+  }
   __syncthreads();
   uint32_t total = 0;
   if (threadIdx.x < mine) {
@@ -370,10 +398,14 @@ __global__ __launch_bounds__(kTileIds) void token_small_kernel(const I* __restri
   }
   if (v0 + mine == rows && threadIdx.x == 0) row_start[rows] = base + all;
   __syncthreads();
-  if (in) {
-    const uint32_t to = counts[wave * range + at] + rank;
-    perm[to] = threadIdx.x;
-    token[to] = static_cast<uint32_t>(id);
+#pragma unroll
+  for (int k = 0; k < kSmallSteps; ++k) {
+    if (!in[k]) continue;
+    const uint32_t rank = ballot_rank(peers[k]);
+    const uint32_t to = own[at[k]];
+    perm[to + rank] = from + k * kWave;
+    token[to + rank] = v0 + at[k];
+    if (rank == 0) own[at[k]] = to + static_cast<uint32_t>(__popcll(peers[k]));
   }
 }
 
@@ -630,7 +662,7 @@ inline size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
 // 35 / 37, 524 288 122 / 52 (the block of the most frequent token's bucket takes the longest: a power law puts
 // a tenth of the ids into it); out of 262 144: 15 / 34, 16 / 40, 36 / 51, 115 / 70.
 struct BucketPlan {
-  bool use;
+  bool use, small;   // small: one kernel
   int bits, shift;   // 2^bits buckets of 2^shift tokens
   int64_t tiles, buckets;
 };
@@ -643,6 +675,7 @@ BucketPlan plan_buckets(int64_t n, int64_t num_rows) {
   b.tiles = ceil_div(n, kTileIds);
   b.buckets = ceil_div(num_rows, int64_t(1) << b.shift);
   b.use = b.bits <= kMaxBucketBits && b.tiles <= kTiles;
+  b.small = n <= kSmallIds;
   return b;
 }
 
@@ -684,13 +717,17 @@ GradWs carve_grad(void* base, int64_t n, int64_t dim, int64_t num_rows) {
 
 // What the sort's launches zero of a dense gradient: as much as memory takes beside them, of a gradient that
 // has at least a row for each position of the batch.  us of the whole gradient with 0 / 20 + 36 / 30 + 50 / 60 +
-// 100 MiB: 2 048 x 1 024 float32 into 32 000 rows 41.4 / 34.4 / 31.3 / 35.0, 12 289 x 1 001 float16 into 50 257
+// 100 MiB: 12 289 x 1 001 float16 into 50 257
 // 47.5 / 40.9 / 38.5 / 43.2, 512 x 1 024 bfloat16 into 32 000 21.0 / 18.7 / 17.8 / 21.7.
 struct EarlyZeros {
   int64_t rows;           // the first rows of the gradient
   ZeroJob first, second;
 };
 constexpr int64_t kZeroFirst = int64_t(30) << 20, kZeroSecond = int64_t(50) << 20;   // bytes
+// beside the one kernel of a small batch with more than one step a wave, which takes longer; with 30 / 40 / 50 MiB:
+// 2 048 x 1 024 float32 into 32 000 rows 32.4 / 31.0 / 31.7, 4 096 x 1 024 bfloat16 23.2 / 22.7 / 23.1; with one
+// step, 1 000 x 1 024 bfloat16, 18.6 / 19.1 / 20.9
+constexpr int64_t kZeroSmall = int64_t(40) << 20;
 
 EarlyZeros plan_zeros(void* out, int64_t out_stride, int64_t n, int64_t num_rows, int64_t dim, int64_t value_bytes,
                       int accumulate, const BucketPlan& b) {
@@ -698,11 +735,12 @@ EarlyZeros plan_zeros(void* out, int64_t out_stride, int64_t n, int64_t num_rows
   z.first.from = z.second.from = ~0u;
   if (!b.use || accumulate || out_stride != dim || (align_of_ptr(out) & 15) != 0 || n > num_rows) return z;
   const int64_t row = dim * value_bytes;
-  const int64_t most = b.tiles == 1 ? kZeroFirst : kZeroFirst + kZeroSecond;
+  const int64_t alone = b.small && b.tiles > 1 ? kZeroSmall : kZeroFirst;   // of the first launch
+  const int64_t most = b.small ? alone : kZeroFirst + kZeroSecond;
   z.rows = (most / row < num_rows ? most / row : num_rows) & ~int64_t(7);   // eight rows are a multiple of 16 bytes
   const int64_t bytes = z.rows * row;
   z.first.p = static_cast<char*>(out);
-  z.first.bytes = bytes < kZeroFirst ? bytes : kZeroFirst;
+  z.first.bytes = bytes < alone ? bytes : alone;
   z.second.p = z.first.p + z.first.bytes;
   z.second.bytes = bytes - z.first.bytes;
   return z;
@@ -719,7 +757,7 @@ template <typename I>
 int sort_tokens(const I* ids, int64_t n, int64_t rows, int64_t num_rows, int64_t padding, const GradWs& w,
                 EarlyZeros& z, const uint32_t** perm, const uint32_t** token, hipStream_t st) {
   const BucketPlan b = plan_buckets(rows, num_rows);
-  if (b.use && b.tiles == 1) {
+  if (b.use && b.small) {
     const dim3 grid(with_zeros(&z.first, b.buckets));
     HADES_LAUNCH((token_small_kernel<I>), grid, dim3(kTileIds), (kTileWaves << b.shift) * sizeof(uint32_t), st, ids, n,
                  num_rows, padding, b.shift, w.perm, w.token, w.row_start, z.first);

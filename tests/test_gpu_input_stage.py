@@ -273,6 +273,34 @@ def test_embed_grad_sorts_every_batch_in_order(cuda_device, n, vocab):
     assert torch.equal(got[small], want[small] + 0.5)
 
 
+@pytest.mark.parametrize("vocab", [2, 257, 40_000, 1 << 20])
+@pytest.mark.parametrize("n", [2047, 2048, 2049, 3073, 4095, 4096, 4097])
+def test_embed_grad_of_a_few_steps_a_wave(cuda_device, n, vocab):
+    """Batches on both sides of one and two kernels.  Every sum of the columns 1 and k mod 61 is a whole number below
+    2^24 (4 097 * 60 = 245 820), so float32 holds each partial sum and the result has to be equal."""
+    k = torch.arange(n) % 61
+    g = torch.stack((torch.ones(n), k.float()), 1)
+    for kind in ("power law", "one token", "two tokens in turn", "last token"):
+        ids = token_ids(n, vocab, 3, 0.1)
+        if kind == "one token":
+            ids.fill_(vocab // 2)
+        elif kind == "two tokens in turn":
+            ids = (torch.arange(n) % 2) * (vocab - 1)
+        elif kind == "last token":
+            ids[n // 2:] = vocab - 1
+        want = torch.zeros((vocab, 2), dtype=torch.float64).index_add_(0, ids[ids >= 0], g[ids >= 0].double())
+        for i in (ids, ids.int()):
+            assert torch.equal(ops.embed_grad(g.cuda(), i.cuda(), vocab).double().cpu(), want), kind
+    # random values: the same bits from run to run
+    ids = token_ids(n, vocab, 5, 0.0)
+    x = torch.randn(n, 96, generator=torch.Generator().manual_seed(n)).cuda()
+    first = ops.embed_grad(x, ids.cuda(), vocab)
+    assert torch.equal(first, ops.embed_grad(x, ids.cuda(), vocab))
+    exact = torch.zeros((vocab, 96), dtype=torch.float64).index_add_(0, ids, x.double().cpu())
+    size = torch.zeros((vocab, 96), dtype=torch.float64).index_add_(0, ids, x.double().abs().cpu())
+    within(first.double().cpu(), exact, size * (n * U))
+
+
 def test_embed_grad_of_no_tokens_and_strided_rows(cuda_device):
     g = rows_of((9, 4, 50), torch.bfloat16, 1).cuda()
     ids = token_ids(9, 6, 2).cuda()
