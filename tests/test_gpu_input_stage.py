@@ -434,6 +434,24 @@ def test_rms_norm_forms_agree(cuda_device):
     assert torch.equal(h, ops.dropout(x, *drop))
 
 
+@pytest.mark.parametrize("rows,cols", [(64, 512), (7, 1001), (33, 4096), (2, 17_000)])
+@pytest.mark.parametrize("group", [0, 128])
+@pytest.mark.parametrize("size", [1.0, 1e-12, 1e-25, 1e28, 1e33])
+def test_rms_norm_8bit_rounds_the_quotient(cuda_device, rows, cols, group, size):
+    """The float32 form gives the same y, so scale and quotient can be looked at alone.  scale: a product and a
+    correction, one step of 2^-23 at most.  q: half a step of e4m3, 2^-4 of the power of two below the value and at
+    least 2^-10, and two steps of float32 beside a tie (the quotient's rounding and the correction's)."""
+    x, w = rows_of((rows, cols), torch.float32, 11).cuda(), (rows_of((cols,), torch.float32, 12) * size).cuda()
+    y = ops.rms_norm(x, w)[0].double().cpu()
+    q, scales, _ = ops.rms_norm_8bit(x, w, group=group)
+    g = group or cols
+    top = torch.nn.functional.pad(y.abs(), (0, -cols % g)).view(rows, -1, g).amax(2)
+    within(scales, top / 448, top / 448 * 2.0 ** -23)
+    u = y / scales.double().cpu().repeat_interleave(g, 1)[:, :cols]
+    half = torch.exp2(u.abs().clamp_min(2.0 ** -6).log2().floor()) * 2.0 ** -4
+    within(q.float(), u, half + u.abs() * 2.0 ** -23)
+
+
 def test_rms_norm_8bit_of_zeros_and_infinities(cuda_device):
     x = rows_of((4, 256), torch.float32, 1)
     x[1] = 0
