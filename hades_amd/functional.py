@@ -126,15 +126,21 @@ class _RmsNorm(torch.autograd.Function):
 
 def embed(weight, ids, scale=1.0, padding_idx=None, dropout=None):
     """ops.embed; weight's gradient is ops.embed_grad (padding_idx gets none)."""
+    if not torch.is_grad_enabled():      # no graph, and nothing that a capture could pull in
+        return ops.embed(weight, ids, scale=scale, dropout=dropout)
     return _Embed.apply(weight, ids, scale, padding_idx, dropout)
 
 
 def dropout(x, p, seed, offset, residual=None):
     """ops.dropout; the gradients are the same mask on the output's gradient, and that gradient itself."""
+    if not torch.is_grad_enabled():
+        return ops.dropout(x, p, seed, offset, residual=residual)
     return _Dropout.apply(x, residual, (p, seed, offset))
 
 
 def rms_norm(x, weight=None, eps=1e-6, residual=None, dropout=None):
     """(y, h) of ops.rms_norm; h is x itself where there is neither residual nor dropout."""
+    if not torch.is_grad_enabled():
+        return ops.rms_norm(x, weight, eps, residual=residual, dropout=dropout)[:2]
     out = _RmsNorm.apply(x, weight, eps, residual, dropout)
     return out if isinstance(out, tuple) else (out, x)

@@ -234,6 +234,34 @@ def test_capture_beside_a_living_eager_graph_is_refused(cuda_device):
     assert torch.equal(out, ops.embed(emb.weight.detach(), ids, dropout=(0.5, 0, 0)))
 
 
+@pytest.mark.parametrize("norm", [True, False])
+def test_capture_without_gradients_beside_a_living_eager_graph(cuda_device, norm):
+    """A captured forward that records no graph has no backward pass to refuse: it gives what the eager call gives,
+    on every replay, while the eager graph of the same leaves lives and is run backward between replays."""
+    emb = dist_emb.TokenEmb(50, 16, torch.float32, dropout=0.5, norm=norm)
+    ids = torch.arange(20, device="cuda")
+    first = lambda out: out[0] if norm else out
+    offset = torch.zeros(1, dtype=torch.int64, device="cuda")
+    alive = first(emb(ids))
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        out = first(emb(ids, offset=offset))
+    assert not out.requires_grad and alive.requires_grad
+    for replay in range(3):
+        offset.fill_(replay)
+        graph.replay()
+        torch.cuda.synchronize()
+        x = emb.weight.detach()
+        if norm:
+            want = ops.rms_norm(ops.embed(x, ids), emb.stage.weight.detach(), dropout=(0.5, 0, replay))[0]
+        else:
+            want = ops.embed(x, ids, dropout=(0.5, 0, replay))
+        assert torch.equal(out, want)
+        alive.sum().backward(retain_graph=True)
+    torch.cuda.synchronize()
+    assert emb.weight.grad is not None
+
+
 def test_offset_tensor_changed_before_backward_is_refused(cuda_device):
     x = rows_of((4, 8), torch.float32, 1).cuda().requires_grad_()
     offset = torch.zeros(1, dtype=torch.int64, device="cuda")
