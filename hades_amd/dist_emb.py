@@ -168,7 +168,9 @@ class InputStage(nn.Module):
         return rows if residual is None else rows + residual
 
     def forward_8bit(self, rows, residual=None, group=0):
-        """(q, scales, h) for an 8-bit product (ops.rms_norm_8bit): no dropout, no gradient."""
+        """(q, scales, h) for an 8-bit product (ops.rms_norm_8bit): no dropout, no gradient.  Goes with norm."""
+        if self.weight is None:
+            raise RuntimeError("forward_8bit goes with norm")
         with torch.no_grad():
             return ops.rms_norm_8bit(rows, self.weight, self.norm_eps, residual=residual, group=group)
 
@@ -202,6 +204,8 @@ class TokenEmb(nn.Module):
 
     def forward_8bit(self, ids, residual=None, group=0):
         """(q, scales, h) of the rows, as InputStage.forward_8bit."""
+        if self.stage.weight is None:
+            raise RuntimeError("forward_8bit goes with norm")
         with torch.no_grad():
             return self.stage.forward_8bit(ops.embed(self.weight, ids, scale=self.scale), residual, group)
 

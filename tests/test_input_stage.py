@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from hades_amd import _lib, ops
+from hades_amd import _lib, dist_emb, ops
 
 NULL = ctypes.c_void_p(0)
 ONE = ctypes.c_void_p(256)      # never dereferenced: the checks fail first
@@ -158,3 +158,11 @@ def test_rms_norm_grad_workspace_query_covers_every_type():
                     short.add(call(nbytes - 256))
             assert 3 in short or not nbytes
             assert nbytes or rows < 1000
+
+
+def test_8bit_rows_go_with_a_norm():
+    # on host tensors: the refusal comes before any launch
+    emb = dist_emb.TokenEmb(10, 8, torch.float32, device="cpu")
+    for call in (lambda: emb.forward_8bit(torch.arange(4)), lambda: emb.stage.forward_8bit(torch.zeros(4, 8))):
+        with pytest.raises(RuntimeError, match="goes with norm"):
+            call()
