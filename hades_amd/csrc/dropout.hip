@@ -6,8 +6,8 @@
 // a function of the value's row and column alone, so the backward pass draws the same one from the
 // same seed and offset, whatever the strides; the gradient of x is this kernel on the output's gradient.
 //
-// Bound by memory: every value is read once and written once.  A thread takes four pieces of eight
-// columns that lie a block apart, so that all its loads are in flight before the first is used.
+// Bound by memory: every value is read once and written once.  A thread takes one piece of eight columns, or
+// two that lie a block apart where 16-bit rows are streamed, with all its loads in flight before the first is used.
 #include "rowvec.h"
 
 namespace hades {

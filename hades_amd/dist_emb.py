@@ -131,7 +131,8 @@ class InputStage(nn.Module):
     training takes the next one (kept with the state dict).  Give the modules of one model, and the
     processes of a data-parallel run, different seeds.  A captured forward needs `offset`, an int64
     tensor of one element on the device that the captured step counts up itself: replays of one number
-    would drop the same values every time."""
+    would drop the same values every time.  A forward that is run again for the backward pass
+    (activation checkpointing) needs an `offset` too, of any kind: its second run would draw another mask."""
 
     def __init__(self, dim, dtype, dropout=0.0, norm=False, norm_eps=1e-6, seed=0, device="cuda"):
         super().__init__()
