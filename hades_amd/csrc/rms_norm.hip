@@ -141,11 +141,13 @@ __device__ __forceinline__ float e4m3_scale(uint32_t m) {
 }
 
 // Eight values in units of `scale`, rounded to e4m3 (nearest even).  scale is the largest magnitude of
-// the group over 448, so a value in its units is at most 448 (1 + 2^-22), which rounds to 448, the type's
-// largest.  Quotients by a refined reciprocal and one correction each: of 4 096 x 8 192 bfloat16 values, groups
+// the group over 448, to half a step: where it is a normal number a value in its units is at most 448 (1 + 2^-22),
+// which rounds to 448, the type's largest.  A subnormal scale of few steps may be too small by a third, and values
+// in its units would reach 672, past the type's range (a NaN); those quotients end at 448.  Quotients by a refined reciprocal and one correction each: of 4 096 x 8 192 bfloat16 values, groups
 // of 128, 2 827 fall to the other side of a tie than in 64 bits; 2 838 with divisions, 3 074 with the reciprocal
 // alone, which takes 170.4 us for 16 384 x 8 192 against 173.  Where the reciprocal would overflow or
-// vanish, or scale is subnormal and coarse, every value is divided; a group of zeros (scale 0) gives zeros.
+// vanish, or scale is subnormal and coarse, every value is divided; a group of zeros (scale 0), or of magnitudes
+// of up to 224 * 2^-149, whose scale rounds to 0, gives zeros.
 __device__ __forceinline__ void store_e4m3(uint8_t* __restrict__ p, f32x8 v, float scale, int valid) {
   f32x8 u;
   if (scale >= 0x1p-60f && scale < 0x1p100f) {
@@ -158,7 +160,10 @@ __device__ __forceinline__ void store_e4m3(uint8_t* __restrict__ p, f32x8 v, flo
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < kPiece; ++j) u[j] = scale > 0.0f ? v[j] / scale : 0.0f;
+    for (int j = 0; j < kPiece; ++j) {
+      const float q = scale > 0.0f ? v[j] / scale : 0.0f;
+      u[j] = q > 448.0f ? 448.0f : (q < -448.0f ? -448.0f : q);   // (a NaN stays one)
+    }
   }
   int lo = 0, hi = 0;
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], lo, false);

@@ -1,0 +1,58 @@
+"""The input stage where its arithmetic or its arguments reach an end: 8-bit scales of the smallest magnitudes,
+outputs that share memory with inputs, the modules' rules, the largest batches."""
+import pytest
+import torch
+
+from hades_amd import ops
+
+pytestmark = pytest.mark.gpu
+STEP = 2.0 ** -149      # float32's smallest number
+
+
+def check_8bit(q, scales, steps, group):
+    """q and scales of rows whose values are `steps` (whole numbers, float64 [rows, cols]) times STEP.
+
+    A scale is top / 448 rounded to a whole number of steps: off by half a step (and by 2^-20 of one, as the quotient
+    by 448 is a product corrected once).  A value in units of its scale is rounded by at most 2^-4 of itself or 2^-10,
+    half the type's smallest step; one above 448 becomes 448, which loses at most 448 half steps.  A scale of 0
+    (largest magnitudes of up to 224 steps) loses the value, at most 224 steps."""
+    assert bool(torch.isfinite(q.float()).all()), "%d values are not finite" % int((~torch.isfinite(q.float())).sum())
+    rows, cols = steps.shape
+    width = group or cols
+    top = steps.abs().reshape(rows, cols // width, width).amax(2)
+    got = scales.cpu().double() / STEP
+    assert bool(((got - top / 448).abs() <= 0.5 * (1 + 2.0 ** -20)).all())
+    unit = torch.repeat_interleave(got, width, 1)
+    value = q.cpu().float().double() * unit
+    bound = 448 * 0.5 * (1 + 2.0 ** -20) + steps.abs() * 2.0 ** -4 + unit * 2.0 ** -10
+    assert bool(((value - steps).abs() <= bound).all())
+
+
+def steps_of(tops, width):
+    """Groups of `width` whole numbers, the largest magnitude of each first (and last, negative)."""
+    parts = torch.arange(width, dtype=torch.float64) / width
+    s = (tops.double()[:, None] * parts).floor()
+    s[:, 0], s[:, -1] = tops, -tops
+    return s
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group", [8, 64])
+def test_8bit_groups_of_the_smallest_magnitudes(cuda_device, dtype, group):
+    # every largest magnitude from 1 to 8 192 steps: scales of 0 to 18 steps.  Rows of ones normalise to 1 - 5e-7,
+    # and a weight of up to 8 192 steps times that rounds to itself
+    for first in range(0, 8192, 1024):
+        tops = torch.arange(first + 1, first + 1025)
+        steps = steps_of(tops, group).reshape(1, -1)
+        x = torch.ones((2, steps.size(1)), dtype=dtype, device="cuda")
+        q, scales, _ = ops.rms_norm_8bit(x, (steps[0] * STEP).float().cuda(), group=group)
+        check_8bit(q, scales, steps.expand(2, -1), group)
+
+
+@pytest.mark.parametrize("cols", [8, 64, 500, 4104, 16416])
+@pytest.mark.parametrize("top", [1, 224, 225, 448, 464, 671, 672, 673, 1119, 448 * 13 + 223, 448 * 14 + 223])
+def test_8bit_rows_of_the_smallest_magnitudes(cuda_device, cols, top):
+    steps = steps_of(torch.tensor([top]), cols)
+    x = torch.ones((3, cols), device="cuda")
+    q, scales, _ = ops.rms_norm_8bit(x, (steps[0] * STEP).float().cuda())
+    check_8bit(q, scales, steps.expand(3, -1), 0)
