@@ -6,7 +6,8 @@ with their gradients for torch.autograd.
     y, h = functional.rms_norm(x, gamma, residual=stream, dropout=(p, seed, offset))
 
 `dropout` = (p, seed, offset) as in ops; an offset tensor must keep its value until the backward pass has
-run (torch's version check raises otherwise).  The backward passes are not differentiable themselves.
+run (torch's version check raises otherwise).  The backward passes are not differentiable themselves, and
+there are no forward-mode derivatives: a tensor that carries a tangent is refused, with gradients on or off.
 
 Graph capture.  A leaf's gradient is accumulated on the stream of the first graph that used the leaf, for
 as long as any graph of it lives.  If that graph was made eagerly on another stream (its output or loss is
@@ -17,6 +18,7 @@ of the same leaf, made through them on another stream, is still alive.
 import weakref
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -124,23 +126,34 @@ class _RmsNorm(torch.autograd.Function):
         return gx if need_x else None, gw, None, gres if need_res else None, None
 
 
+def _plain(*tensors):
+    """Whether a call has no derivative to record: gradients are off and no tensor carries a forward-mode
+    tangent (autograd.Function, which has no rule for tangents here, refuses those)."""
+    if torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and unpack_dual(t).tangent is not None:
+            return False
+    return True
+
+
 def embed(weight, ids, scale=1.0, padding_idx=None, dropout=None):
     """ops.embed; weight's gradient is ops.embed_grad (padding_idx gets none)."""
-    if not torch.is_grad_enabled():      # no graph, and nothing that a capture could pull in
+    if _plain(weight):      # no graph, and nothing that a capture could pull in
         return ops.embed(weight, ids, scale=scale, dropout=dropout)
     return _Embed.apply(weight, ids, scale, padding_idx, dropout)
 
 
 def dropout(x, p, seed, offset, residual=None):
     """ops.dropout; the gradients are the same mask on the output's gradient, and that gradient itself."""
-    if not torch.is_grad_enabled():
+    if _plain(x, residual):
         return ops.dropout(x, p, seed, offset, residual=residual)
     return _Dropout.apply(x, residual, (p, seed, offset))
 
 
 def rms_norm(x, weight=None, eps=1e-6, residual=None, dropout=None):
     """(y, h) of ops.rms_norm; h is x itself where there is neither residual nor dropout."""
-    if not torch.is_grad_enabled():
+    if _plain(x, weight, residual):
         return ops.rms_norm(x, weight, eps, residual=residual, dropout=dropout)[:2]
     out = _RmsNorm.apply(x, weight, eps, residual, dropout)
     return out if isinstance(out, tuple) else (out, x)

@@ -2,8 +2,9 @@
 outputs that share memory with inputs, the modules' rules, the largest batches."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from hades_amd import ops
+from hades_amd import functional, ops
 
 pytestmark = pytest.mark.gpu
 STEP = 2.0 ** -149      # float32's smallest number
@@ -56,3 +57,21 @@ def test_8bit_rows_of_the_smallest_magnitudes(cuda_device, cols, top):
     x = torch.ones((3, cols), device="cuda")
     q, scales, _ = ops.rms_norm_8bit(x, (steps[0] * STEP).float().cuda())
     check_8bit(q, scales, steps.expand(3, -1), 0)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_tangents_are_refused(cuda_device, grad):
+    """A tangent never gets lost: with gradients on or off, autograd refuses a tensor that carries one."""
+    t = torch.ones((4, 8), device="cuda")
+    w = torch.ones(8, device="cuda")
+    ids = torch.arange(4, device="cuda")
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        x, g = forward_ad.make_dual(t, t), forward_ad.make_dual(w, w)
+        for call in (lambda: functional.embed(x, ids), lambda: functional.dropout(x, 0.5, 1, 0),
+                     lambda: functional.dropout(t, 0.5, 1, 0, residual=x), lambda: functional.rms_norm(x, w),
+                     lambda: functional.rms_norm(t, g), lambda: functional.rms_norm(t, w, residual=x),
+                     lambda: functional.rms_norm(t, residual=x, dropout=(0.5, 1, 0))):
+            with pytest.raises(NotImplementedError, match="jvp"):
+                call()
+        # and one that carries none is served inside the level as outside
+        assert torch.equal(functional.embed(t, ids), t) and torch.equal(functional.dropout(t, 1.0, 1, 0, residual=t), t)
