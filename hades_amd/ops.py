@@ -1025,7 +1025,8 @@ def _weight_type(weight, x, cols, name):
 
 
 def _norm_args(x, weight, residual, dropout, dev, h_out):
-    """(type, row stride, columns, residual's stride, weight's type, dropout, h) of a norm's forward call"""
+    """(type, row stride, columns, residual's stride, weight's type, dropout, h, what the kernel stores h to: None
+    where h is x as it is) of a norm's forward call"""
     dtype, stride = _row_type(x, "x"), _row_stride(x, "x", dev)
     cols = x.size(-1)
     if cols < 1:
@@ -1038,10 +1039,11 @@ def _norm_args(x, weight, residual, dropout, dev, h_out):
         res_stride = _row_stride(residual, "residual", dev)
     if weight is not None:
         weight_type = _weight_type(weight, x, cols, "x")
-    h = x
+    h, h_ptr = x, None
     if residual is not None or dropout is not None or h_out is not None:
         h = _out_like(x, h_dtype, h_out, "h_out")
-    return dtype, stride, cols, res_stride, weight_type, _drop_args(dropout, dev), h
+        h_ptr = h.data_ptr()
+    return dtype, stride, cols, res_stride, weight_type, _drop_args(dropout, dev), h, h_ptr
 
 
 def rms_norm(x, weight=None, eps=1e-6, residual=None, dropout=None, out=None, h_out=None):
@@ -1049,13 +1051,13 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, dropout=None, out=None, h_
     Returns (y, h, rstd): y of x's type, h of the residual's (x itself where there is neither residual
     nor dropout), rstd = 1 / sqrt(...) float32 of shape x.shape[:-1], for rms_norm_grad.  The norm is
     taken of h before its rounding.  residual and weight have x's type or float32; weight None: ones.
-    `h_out` may be residual."""
+    `h_out` may be residual or x."""
     dev, stream = _enter(x, "x")
-    dtype, stride, cols, res_stride, weight_type, drop, h = _norm_args(x, weight, residual, dropout, dev, h_out)
+    dtype, stride, cols, res_stride, weight_type, drop, h, h_ptr = _norm_args(x, weight, residual, dropout, dev, h_out)
     y = _out_like(x, x.dtype, out)
     rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
     _lib.call("hades_rms_norm", x.data_ptr(), stride, _ptr_or_none(residual), res_stride, _ptr_or_none(weight),
-              y.data_ptr(), None, None if h is x else h.data_ptr(), rstd.data_ptr(), rstd.numel(), cols, dtype,
+              y.data_ptr(), None, h_ptr, rstd.data_ptr(), rstd.numel(), cols, dtype,
               _ROW_TYPES[h.dtype], weight_type, 0, float(eps), *drop, stream)
     return y, h, rstd
 
@@ -1066,14 +1068,14 @@ def rms_norm_8bit(x, weight=None, eps=1e-6, residual=None, group=0, dropout=None
     one for the row), scale = max|y| / 448.  A group of zeros has scale 0; one with an infinity or a NaN
     has a scale that is one too."""
     dev, stream = _enter(x, "x")
-    dtype, stride, cols, res_stride, weight_type, drop, h = _norm_args(x, weight, residual, dropout, dev, h_out)
+    dtype, stride, cols, res_stride, weight_type, drop, h, h_ptr = _norm_args(x, weight, residual, dropout, dev, h_out)
     _check(group == 0 or (8 <= group <= 512 and group & (group - 1) == 0),
            "group must be 0 or a power of two in [8, 512]")
     q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
     groups = 1 if group == 0 else -(-cols // group)
     scales = x.new_empty((*x.shape[:-1], groups), dtype=torch.float32)
     _lib.call("hades_rms_norm", x.data_ptr(), stride, _ptr_or_none(residual), res_stride, _ptr_or_none(weight),
-              q.data_ptr(), scales.data_ptr(), None if h is x else h.data_ptr(), None, scales.numel() // groups, cols,
+              q.data_ptr(), scales.data_ptr(), h_ptr, None, scales.numel() // groups, cols,
               dtype, _ROW_TYPES[h.dtype], weight_type, int(group), float(eps), *drop, stream)
     return q, scales, h
 

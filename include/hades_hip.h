@@ -664,7 +664,7 @@ int hades_dropout(const void* x, int64_t x_stride, const void* residual, int64_t
 
 /* h = residual + dropout(x); rstd = 1 / sqrt(mean(h^2) + eps); y = h * rstd * weight.
  * residual (type stream_dtype: dtype or HADES_F32), weight (weight_dtype: dtype or HADES_F32; NULL: ones), h
- * (stream_dtype) and rstd may be NULL.  h may be residual where its rows are dense.  With scales != NULL, y
+ * (stream_dtype) and rstd may be NULL.  h may be residual, or x, where its rows are dense.  With scales != NULL, y
  * is written as OCP e4m3 bytes in units of scales[rows][ceil(cols / group)], scale = max|y| / 448 over
  * `group` columns (a power of two in [8, 512], or 0: the whole row); a group of zeros (or of magnitudes of up
  * to 224 * 2^-149, whose scale rounds to 0) has scale 0 and bytes 0, one with an infinity or a NaN a scale that is

@@ -75,3 +75,31 @@ def test_forward_mode_tangents_are_refused(cuda_device, grad):
                 call()
         # and one that carries none is served inside the level as outside
         assert torch.equal(functional.embed(t, ids), t) and torch.equal(functional.dropout(t, 1.0, 1, 0, residual=t), t)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("which", ["x", "residual", "view of x"])
+@pytest.mark.parametrize("cols", [8, 333, 4096, 9000, 16500])      # every form of the kernel
+def test_norm_in_place(cuda_device, cols, which, eight):
+    """h_out may be x or the residual: h lands there, and everything is what separate outputs give."""
+    g = torch.Generator().manual_seed(cols)
+    x, res = (torch.randn((5, cols), generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    w = torch.randn(cols, generator=g).cuda()
+
+    def call(x, res, drop, **kw):
+        if eight:
+            q, scales, h = ops.rms_norm_8bit(x, w, residual=res, group=64, dropout=drop, **kw)
+            return q.view(torch.uint8), scales, h
+        return ops.rms_norm(x, w, residual=res, dropout=drop, **kw)
+    for residual, drop in ((res, None), (res, (0.3, 1, 2)), (None, (0.3, 1, 2)), (None, None)):
+        if which == "residual" and residual is None:
+            continue
+        want = call(x, residual, drop)
+        mine, theirs = x.clone(), None if residual is None else residual.clone()
+        into = theirs if which == "residual" else (mine if which == "x" else mine.view(5, cols))
+        got = call(mine, theirs, drop, h_out=into)
+        h = got[1] if not eight else got[2]
+        assert h is into
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        assert torch.equal(theirs if which == "residual" else mine, want[1] if not eight else want[2])
