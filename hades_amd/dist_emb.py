@@ -125,7 +125,8 @@ class DistEmbeddingTensor:
 
 class InputStage(nn.Module):
     """What rows go through on their way into a model: h = residual + dropout(rows), and with `norm`
-    y = h / sqrt(mean(h^2) + norm_eps) * weight.
+    y = h / sqrt(mean(h^2) + norm_eps) * weight.  The residual has the rows' shape, and their type or float32,
+    which h then has too - in training and in evaluation, with norm and without.
 
     The masks of a module are drawn from (seed, offset); without an explicit offset every forward call in
     training takes the next one (kept with the state dict).  Give the modules of one model, and the
@@ -161,6 +162,8 @@ class InputStage(nn.Module):
 
     def forward(self, rows, residual=None, offset=None):
         """h, or with norm the pair (y, h)."""
+        if residual is not None and (residual.shape != rows.shape or residual.dtype not in (rows.dtype, torch.float32)):
+            raise RuntimeError("residual must have the rows' shape, and their dtype or float32")
         drop = self.draw(offset)
         if self.weight is not None:
             return _functional.rms_norm(rows, self.weight, self.norm_eps, residual=residual, dropout=drop)

@@ -82,18 +82,26 @@ class _Embed(torch.autograd.Function):
         return grad, None, None, None, None
 
 
+def _as_stream(x, residual):
+    """x, widened where 16-bit rows go onto a float32 residual stream (ops.dropout takes rows of one type)."""
+    if residual is not None and residual.dtype == torch.float32 and x.dtype in (torch.float16, torch.bfloat16):
+        return x.float()
+    return x
+
+
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, dropout):
         _note(ctx, x, residual)
         _keep_drop(ctx, dropout)
-        return ops.dropout(x, *dropout, residual=residual)
+        ctx.x_dtype = x.dtype
+        return ops.dropout(_as_stream(x, residual), *dropout, residual=residual)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         _, drop = _kept(ctx)
-        gx = ops.dropout_grad(grad.contiguous(), *drop) if ctx.needs_input_grad[0] else None
+        gx = ops.dropout_grad(grad.contiguous(), *drop).to(ctx.x_dtype) if ctx.needs_input_grad[0] else None
         return gx, grad if ctx.needs_input_grad[1] else None, None
 
 
@@ -145,9 +153,10 @@ def embed(weight, ids, scale=1.0, padding_idx=None, dropout=None):
 
 
 def dropout(x, p, seed, offset, residual=None):
-    """ops.dropout; the gradients are the same mask on the output's gradient, and that gradient itself."""
+    """ops.dropout, and of 16-bit rows onto a float32 residual too, with a float32 sum; the gradients are the same mask
+    on the output's gradient, and that gradient itself."""
     if _plain(x, residual):
-        return ops.dropout(x, p, seed, offset, residual=residual)
+        return ops.dropout(_as_stream(x, residual), p, seed, offset, residual=residual)
     return _Dropout.apply(x, residual, (p, seed, offset))
 
 

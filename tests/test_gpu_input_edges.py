@@ -4,7 +4,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from hades_amd import functional, ops
+from hades_amd import dist_emb, functional, ops
 
 pytestmark = pytest.mark.gpu
 STEP = 2.0 ** -149      # float32's smallest number
@@ -103,3 +103,41 @@ def test_norm_in_place(cuda_device, cols, which, eight):
         for a, b in zip(got, want):
             assert torch.equal(a, b)
         assert torch.equal(theirs if which == "residual" else mine, want[1] if not eight else want[2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("norm", [False, True])
+def test_float32_residual_in_training_and_evaluation(cuda_device, dtype, norm):
+    """16-bit rows onto a float32 stream: one rule whatever the mode, and gradients of both."""
+    n, dim, drop = 70, 40, (0.25, 9, 3)
+    g = torch.Generator().manual_seed(1)
+    x, res = torch.randn((n, dim), generator=g).to(dtype).cuda(), torch.randn((n, dim), generator=g).cuda()
+    c = torch.randn((n, dim), generator=g).cuda()
+    stage = dist_emb.InputStage(dim, dtype, dropout=drop[0], norm=norm, seed=drop[1])
+    x.requires_grad_(), res.requires_grad_()
+    h = stage(x, res, offset=drop[2])
+    h = h[1] if norm else h
+    h.backward(c)
+    masked = ops.dropout(x.detach().float(), *drop)
+    assert h.dtype == torch.float32 and torch.equal(h, masked + res)     # the sum's one rounding, in either order
+    assert torch.equal(res.grad, c) and x.grad.dtype == dtype and torch.equal(x.grad, ops.dropout_grad(c, *drop).to(dtype))
+    with torch.no_grad():
+        again = stage(x, res, offset=drop[2])
+        assert torch.equal(again[1] if norm else again, h)
+        stage.eval()
+        plain = stage(x, res)
+        assert torch.equal(plain[1] if norm else plain, x.float() + res)
+
+
+@pytest.mark.parametrize("training", [True, False])
+@pytest.mark.parametrize("p", [0.0, 0.5])
+@pytest.mark.parametrize("norm", [False, True])
+def test_residuals_that_no_mode_takes(cuda_device, training, p, norm):
+    stage = dist_emb.InputStage(8, torch.float32, dropout=p, norm=norm, seed=1).train(training)
+    x = torch.ones((4, 8), device="cuda")
+    for bad in (x[:1], x[0], x.bfloat16(), x.double(), torch.ones((2, 4, 8), device="cuda")):
+        with pytest.raises(RuntimeError, match="residual must have"):
+            stage(x, bad)
+    with pytest.raises(RuntimeError, match="residual must have"):
+        stage(x.bfloat16(), x.half())
+    assert stage(x, x) is not None
