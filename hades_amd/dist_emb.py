@@ -20,6 +20,10 @@ What a model does with its rows first - dropout, the addition to a residual stre
 norm, the rounding to 8 bits - is InputStage, which DistEmb (dropout=, norm=) and TokenEmb (a vocabulary
 table in HBM with a dense gradient) share.  None of it has a counterpart in the reference.
 """
+import itertools
+import threading
+import weakref
+
 import torch
 import torch.nn as nn
 
@@ -123,31 +127,53 @@ class DistEmbeddingTensor:
         return self._fetch_only(ids.to(self._device).long())
 
 
+_stages = weakref.WeakSet()      # the living InputStages of the process
+_stages_lock = threading.Lock()
+
+
 class InputStage(nn.Module):
     """What rows go through on their way into a model: h = residual + dropout(rows), and with `norm`
     y = h / sqrt(mean(h^2) + norm_eps) * weight.  The residual has the rows' shape, and their type or float32,
     which h then has too - in training and in evaluation, with norm and without.
 
     The masks of a module are drawn from (seed, offset); without an explicit offset every forward call in
-    training takes the next one (kept with the state dict).  Give the modules of one model, and the
-    processes of a data-parallel run, different seeds.  A captured forward needs `offset`, an int64
+    training takes the next one.  Without an explicit seed a module takes, when it first draws a mask, the lowest
+    number that no living module of the process has for a seed, so that the modules of one model draw different
+    masks; a copy made after that draws what its original draws.  Offset and seed are kept with the state dict (a
+    seed given here is not replaced by the dict's).  Give the processes of a data-parallel run different seeds, for
+    each of their modules: their numbers would be the same.  A captured forward needs `offset`, an int64
     tensor of one element on the device that the captured step counts up itself: replays of one number
     would drop the same values every time.  A forward that is run again for the backward pass
     (activation checkpointing) needs an `offset` too, of any kind: its second run would draw another mask."""
 
-    def __init__(self, dim, dtype, dropout=0.0, norm=False, norm_eps=1e-6, seed=0, device="cuda"):
+    def __init__(self, dim, dtype, dropout=0.0, norm=False, norm_eps=1e-6, seed=None, device="cuda"):
         super().__init__()
         if not 0.0 <= dropout <= 1.0:
             raise RuntimeError("dropout must lie in [0, 1]")
-        self.dropout, self.norm_eps, self.seed = float(dropout), float(norm_eps), int(seed)
+        self.dropout, self.norm_eps = float(dropout), float(norm_eps)
+        self.seed, self._seed_given = None if seed is None else int(seed), seed is not None
         self.weight = nn.Parameter(torch.ones(dim, dtype=dtype, device=device)) if norm else None
         self._calls = 0
+        _stages.add(self)
+
+    def __setstate__(self, state):      # of a copy, or of one pickled when every module had a seed
+        super().__setstate__(state)
+        self.__dict__.setdefault("_seed_given", True)
+        _stages.add(self)
 
     def get_extra_state(self):
-        return {"calls": self._calls}
+        return {"calls": self._calls, "seed": self.seed}
 
     def set_extra_state(self, state):
         self._calls = int(state["calls"])
+        if not self._seed_given and state.get("seed") is not None:
+            self.seed = int(state["seed"])
+
+    def _take_seed(self):
+        with _stages_lock:
+            if self.seed is None:
+                taken = {stage.seed for stage in _stages}
+                self.seed = next(n for n in itertools.count() if n not in taken)
 
     def draw(self, offset=None):
         """(p, seed, offset) of this forward call's mask, or None outside training."""
@@ -158,6 +184,8 @@ class InputStage(nn.Module):
                 raise RuntimeError("a captured forward with dropout needs an offset tensor on the device")
             offset = self._calls
             self._calls += 1
+        if self.seed is None:
+            self._take_seed()
         return self.dropout, self.seed, offset
 
     def forward(self, rows, residual=None, offset=None):
@@ -187,7 +215,7 @@ class TokenEmb(nn.Module):
     `padding_idx` is used but gets no gradient."""
 
     def __init__(self, num_rows, dim, dtype=torch.bfloat16, scale=1.0, padding_idx=None, dropout=0.0, norm=False,
-                 norm_eps=1e-6, seed=0, weight=None, device="cuda"):
+                 norm_eps=1e-6, seed=None, weight=None, device="cuda"):
         super().__init__()
         if weight is None:
             weight = torch.empty((num_rows, dim), dtype=torch.float32).normal_(0.0, dim ** -0.5).to(dtype)
@@ -222,7 +250,7 @@ class DistEmb(nn.Module):
     def __init__(self, num_nodes, emb_dim, emb_dtype, name, cache_rate=0.3, idx_dtype=None,
                  local_rank=None, local_trainer_num=None, hotness_list=None, hot_threshold=150,
                  part_book=None, cache_server_addr=None, cache_server_port=None, *, dropout=0.0,
-                 norm=False, norm_eps=1e-6, seed=0, **kw):
+                 norm=False, norm_eps=1e-6, seed=None, **kw):
         super().__init__()
         self.emb_dim = emb_dim
         self.stage = InputStage(emb_dim, emb_dtype, dropout, norm, norm_eps, seed,

@@ -141,3 +141,17 @@ def test_residuals_that_no_mode_takes(cuda_device, training, p, norm):
     with pytest.raises(RuntimeError, match="residual must have"):
         stage(x.bfloat16(), x.half())
     assert stage(x, x) is not None
+
+
+def test_layers_without_seeds_draw_different_masks(cuda_device):
+    """A model of default modules: no two of its layers drop the same values, in any step."""
+    layers = [dist_emb.InputStage(512, torch.float32, dropout=0.5) for _ in range(3)]
+    table = dist_emb.TokenEmb(64, 512, torch.float32, dropout=0.5, weight=torch.ones(64, 512))
+    ids, x = torch.arange(64, device="cuda"), torch.ones((64, 512), device="cuda")
+    masks = []
+    for _ in range(2):
+        masks += [layer(x) != 0 for layer in layers] + [table(ids) != 0]
+    for i, a in enumerate(masks):
+        for b in masks[:i]:
+            # independent halves agree in half of 32 768 places, five standard deviations are 453
+            assert abs(int((a == b).sum()) - 16384) < 453
