@@ -12,8 +12,9 @@ there are no forward-mode derivatives: a tensor that carries a tangent is refuse
 Graph capture.  A leaf's gradient is accumulated on the stream of the first graph that used the leaf, for
 as long as any graph of it lives.  If that graph was made eagerly on another stream (its output or loss is
 still referenced), a backward pass under capture would pull that stream into the capture, which ends the
-process on the default stream.  The functions here refuse that: under capture they raise if an eager graph
-of the same leaf, made through them on another stream, is still alive.
+process on the default stream.  A graph that was itself captured on another stream would pull in that one.  The
+functions here refuse both: under capture they raise if a graph of the same leaf, made through them on another
+stream, is still alive.
 """
 import weakref
 
@@ -27,8 +28,8 @@ _graphs = {}      # id of a leaf -> (weak reference to it, weak set of the graph
 
 
 def _note(ctx, *leaves):
-    """Records this call's graph with the leaves it uses; refuses a capture beside an eager graph."""
-    capturing = torch.cuda.is_current_stream_capturing()
+    """Records this call's graph with the leaves it uses; refuses a capture beside a graph of another stream."""
+    capturing = ctx.captured = torch.cuda.is_current_stream_capturing()
     ctx.stream = torch.cuda.current_stream().cuda_stream
     for t in leaves:
         if t is None or not t.requires_grad or not t.is_leaf:
@@ -37,9 +38,15 @@ def _note(ctx, *leaves):
         entry = _graphs.get(key)
         if entry is None or entry[0]() is not t:
             entry = _graphs[key] = (weakref.ref(t, lambda r, key=key: _forget(key, r)), weakref.WeakSet())
-        if capturing and any(c.stream != ctx.stream for c in entry[1]):
-            raise RuntimeError("an eager graph of the same leaf lives on another stream: drop its output and loss "
-                               "before capturing (a backward pass under capture would end the process)")
+        if capturing:
+            for other in entry[1]:
+                if other.stream == ctx.stream:
+                    continue
+                if other.captured:
+                    raise RuntimeError("a graph of the same leaf that was captured on another stream is alive: capture "
+                                       "on that stream, or drop its output and loss before capturing")
+                raise RuntimeError("an eager graph of the same leaf lives on another stream: drop its output and loss "
+                                   "before capturing (a backward pass under capture would end the process)")
         entry[1].add(ctx)
 
 

@@ -155,3 +155,24 @@ def test_layers_without_seeds_draw_different_masks(cuda_device):
         for b in masks[:i]:
             # independent halves agree in half of 32 768 places, five standard deviations are 453
             assert abs(int((a == b).sum()) - 16384) < 453
+
+
+def test_captures_of_one_leaf_on_two_streams(cuda_device):
+    """Beside a graph that was captured on another stream the refusal says so; on the same stream it is served."""
+    w = torch.arange(32.0, device="cuda").reshape(4, 8).requires_grad_()
+    ids = torch.tensor([3, 1], device="cuda")
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    with torch.cuda.graph(graphs[0], stream=first):
+        a = functional.embed(w, ids)
+    with pytest.raises(RuntimeError, match="captured on another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=second):
+            functional.embed(w, ids)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graphs[1], stream=first):
+        b = functional.embed(w, ids, 2.0)
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, w.detach()[ids]) and torch.equal(b, 2 * w.detach()[ids])
