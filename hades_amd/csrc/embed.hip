@@ -791,16 +791,35 @@ int sort_tokens(const I* ids, int64_t n, int64_t rows, int64_t num_rows, int64_t
   return HADES_OK;
 }
 
+// Blocks of the sums and of the zeros behind them, and whether their launch and the join's fit HIP's limits: fewer
+// than 2^32 threads along a dimension, at most 65 535 blocks along y.  (The join's x has 64 threads a chunk: below
+// 2^31, as a batch of 2^28 positions or more has chunks of 32.)
+struct SumGrid {
+  int64_t sum_blocks, zero_blocks;
+  bool fits;
+};
+
+SumGrid plan_sum_grid(const GradPlan& p, int64_t zero_units) {
+  SumGrid g;
+  g.sum_blocks = ceil_div(p.chunks * p.slices * p.group, kThreads);
+  g.zero_blocks = ceil_div(zero_units, int64_t(kThreads) * kZeroUnits);
+  g.fits = g.sum_blocks + g.zero_blocks < (int64_t(1) << 24) && (p.chunks <= p.reach || p.slices <= 65535);
+  return g;
+}
+
+// 16-byte units of the rows that the sums' launch zeroes (where their tokens do not occur); one more unit a row
+// where a row may begin inside one
+int64_t zero_units_of_row(const void* out, int64_t out_stride, int64_t dim, int64_t value_bytes) {
+  const int64_t unit = 16 / value_bytes;
+  const bool aligned = (align_of_ptr(out) & 15) == 0 && out_stride % unit == 0;
+  return ceil_div(dim, unit) + (aligned ? 0 : 1);
+}
+
 template <typename T, typename O, int G, int CH>
-int launch_sums(GradArgs<T, O>& a, const GradPlan& p, hipStream_t st) {
-  const int64_t sum_blocks = ceil_div(p.chunks * p.slices * G, kThreads);
-  const int64_t zero_blocks = a.accumulate ? 0 : ceil_div(a.zero_units, int64_t(kThreads) * kZeroUnits);
-  HADES_REQUIRE(p.chunks * p.slices < (int64_t(1) << 31) && sum_blocks + zero_blocks < (int64_t(1) << 24) &&
-                    p.chunks * p.slices < (int64_t(1) << 24),
-                "embed_grad: too many values for one call");
-  a.sum_blocks = static_cast<unsigned>(sum_blocks);
-  if (sum_blocks + zero_blocks > 0)
-    HADES_LAUNCH((embed_grad_sum_kernel<T, O, G, CH>), dim3(static_cast<unsigned>(sum_blocks + zero_blocks)),
+int launch_sums(GradArgs<T, O>& a, const GradPlan& p, const SumGrid& g, hipStream_t st) {
+  a.sum_blocks = static_cast<unsigned>(g.sum_blocks);
+  if (g.sum_blocks + g.zero_blocks > 0)
+    HADES_LAUNCH((embed_grad_sum_kernel<T, O, G, CH>), dim3(static_cast<unsigned>(g.sum_blocks + g.zero_blocks)),
                  dim3(kThreads), 0, st, a);
   if (p.chunks > p.reach)   // (there are no long tokens otherwise)
     HADES_LAUNCH((embed_grad_join_kernel<T, O, G, CH>),
@@ -812,7 +831,8 @@ int launch_sums(GradArgs<T, O>& a, const GradPlan& p, hipStream_t st) {
 template <typename T, typename O>
 int launch_grad(const void* grad, int64_t grad_stride, const uint32_t* perm, const uint32_t* token, void* out,
                 int64_t out_stride, int64_t n, int64_t num_rows, int64_t dim, const GradPlan& p, const GradWs& w,
-                int accumulate, int64_t zero_from, const DropArgs& drop, hipStream_t st) {
+                int accumulate, int64_t zero_from, int64_t zero_row, int64_t zero_units, const SumGrid& grid,
+                const DropArgs& drop, hipStream_t st) {
   GradArgs<T, O> a;
   a.grad = static_cast<const T*>(grad);
   a.perm = perm;
@@ -830,20 +850,16 @@ int launch_grad(const void* grad, int64_t grad_stride, const uint32_t* perm, con
   a.reach = p.reach;
   a.accumulate = accumulate;
   a.once = streamed(n * dim * static_cast<int64_t>(sizeof(T)));
-  // one more unit where a row may begin inside one
-  constexpr int64_t kUnit = 16 / sizeof(O);
-  const bool aligned = (align_of_ptr(out) & 15) == 0 && out_stride % kUnit == 0;
-  const int64_t units = ceil_div(dim, kUnit) + (aligned ? 0 : 1);
-  a.per_row = FastDiv(static_cast<uint32_t>(units));
+  a.per_row = FastDiv(static_cast<uint32_t>(zero_row));
   a.per_chunk = FastDiv(static_cast<uint32_t>(p.slices));
-  a.zero_units = (num_rows - zero_from) * units;
+  a.zero_units = zero_units;
   a.zero_from = zero_from;
   a.drop = drop;
-#define HADES_SUMS(G_)                                                   \
-  do {                                                                   \
-    if (p.chunk == kChunkLong) return launch_sums<T, O, G_, kChunkLong>(a, p, st); \
-    if (p.chunk == kChunk) return launch_sums<T, O, G_, kChunk>(a, p, st);         \
-    return launch_sums<T, O, G_, kChunkShort>(a, p, st);                 \
+#define HADES_SUMS(G_)                                                                   \
+  do {                                                                                   \
+    if (p.chunk == kChunkLong) return launch_sums<T, O, G_, kChunkLong>(a, p, grid, st); \
+    if (p.chunk == kChunk) return launch_sums<T, O, G_, kChunk>(a, p, grid, st);         \
+    return launch_sums<T, O, G_, kChunkShort>(a, p, grid, st);                           \
   } while (0)
   switch (p.group) {
     case 8: HADES_SUMS(8);
@@ -916,8 +932,13 @@ int hades_embed_grad(const void* grad, int64_t grad_stride, const void* ids, int
   hipStream_t st = static_cast<hipStream_t>(stream);
   const GradPlan plan = plan_grad(rows, dim);
   const uint32_t *perm = nullptr, *token = nullptr;
-  EarlyZeros zeros = plan_zeros(out, out_stride, rows, num_rows, dim, out_dtype == HADES_F32 ? 4 : 2, accumulate,
+  const int64_t value_bytes = out_dtype == HADES_F32 ? 4 : 2;
+  EarlyZeros zeros = plan_zeros(out, out_stride, rows, num_rows, dim, value_bytes, accumulate,
                                 plan_buckets(rows, num_rows));
+  const int64_t zero_row = zero_units_of_row(out, out_stride, dim, value_bytes);
+  const int64_t zero_units = accumulate ? 0 : (num_rows - zeros.rows) * zero_row;
+  const SumGrid grid = plan_sum_grid(plan, zero_units);
+  HADES_REQUIRE(grid.fits, "embed_grad: too many values for one call");   // (before the first launch)
   const int rc = itype == HADES_I64
                      ? sort_tokens(static_cast<const int64_t*>(ids), n, rows, num_rows, padding_idx, w, zeros, &perm,
                                    &token, st)
@@ -926,7 +947,7 @@ int hades_embed_grad(const void* grad, int64_t grad_stride, const void* ids, int
   if (rc != HADES_OK) return rc;
 #define HADES_GRAD(T_, O_)                                                                               \
   return launch_grad<T_, O_>(grad, grad_stride, perm, token, out, out_stride, n, num_rows, dim, plan, w, \
-                             accumulate != 0, zeros.rows, drop, st)
+                             accumulate != 0, zeros.rows, zero_row, zero_units, grid, drop, st)
   if (dtype == HADES_F32) HADES_GRAD(float, float);
   if (dtype == HADES_F16) {
     if (out_dtype == HADES_F16) HADES_GRAD(f16, f16);

@@ -649,7 +649,10 @@ int hades_embed(const void* weight, int64_t weight_stride, int64_t num_rows, con
  * for tokens that do not occur); with accumulate != 0 the sum is added to out[v, :] and the rows of
  * tokens that do not occur stay as they are.  Ids outside [0, num_rows) and padding_idx (negative: none)
  * have no gradient.  out_dtype is dtype or HADES_F32.  Sums in float32, their order fixed by (n, dim) and
- * the ids.  workspace: 256-byte aligned, needs no initialisation. */
+ * the ids.  n < 2^30, num_rows and dim < 2^31; a call is refused, before it launches anything, where a dense
+ * gradient has about 2^33 16-byte units (137 GB) or more, where a batch of more than 64 positions has rows of more
+ * than 65 535 * 512 values, or where n * dim reaches about 2^40.  workspace: 256-byte aligned, needs no
+ * initialisation. */
 size_t hades_embed_grad_workspace_bytes(int64_t n, int64_t dim, int64_t num_rows);
 int hades_embed_grad(const void* grad, int64_t grad_stride, const void* ids, int64_t n, void* out,
                      int64_t out_stride, int64_t num_rows, int64_t dim, int dtype, int out_dtype, int itype,

@@ -176,3 +176,23 @@ def test_captures_of_one_leaf_on_two_streams(cuda_device):
             graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(a, w.detach()[ids]) and torch.equal(b, 2 * w.detach()[ids])
+
+
+def test_embed_grad_of_more_than_2_to_29_positions(cuda_device):
+    """A batch past 2^29 positions, whole numbers: every partial sum stays below 2^24, so the result has to be equal."""
+    n, vocab, dim = (1 << 29) + 37, 1009, 8
+    ids = torch.arange(n, dtype=torch.int32, device="cuda") % vocab
+    ids[-5:] = -1
+    rows = torch.arange(8, device="cuda")[:, None] + torch.arange(dim, device="cuda") - 7       # -7 .. 7, by position % 8
+    grad = rows.to(torch.bfloat16).repeat((n + 7) // 8, 1)[:n]
+    got = ops.embed_grad(grad, ids, vocab, out_dtype=torch.float32)
+    # the positions of token v: v, v + vocab, ...: eight in a row (vocab is odd) meet each remainder once
+    count = torch.zeros((vocab, 8), dtype=torch.int64, device="cuda")
+    for first in range(0, n, 1 << 26):
+        last = min(first + (1 << 26), n)
+        part = ids[first:last].long()
+        key = part * 8 + torch.arange(first, last, device="cuda") % 8
+        count += torch.bincount(key[part >= 0], minlength=8 * vocab).view(vocab, 8)
+    want = count.double() @ rows.double()
+    assert float(count.sum()) == n - 5 and float(want.abs().max()) < 2 ** 24
+    assert torch.equal(got.double(), want)

@@ -1,13 +1,14 @@
 """The input stage's host logic at its edges (no GPU): the seeds that modules draw their masks from, and refusals that
 come before the first launch."""
 import copy
+import ctypes
 import gc
 import pickle
 
 import pytest
 import torch
 
-from hades_amd import dist_emb
+from hades_amd import _lib, dist_emb
 
 
 def stage(**kw):
@@ -77,3 +78,14 @@ def test_residuals_that_no_mode_takes(training):
     for bad in (x[:1], x[0], x.bfloat16(), x.double()):
         with pytest.raises(RuntimeError, match="residual must have"):
             module(x, bad, offset=0)
+
+
+@pytest.mark.parametrize("n,num_rows,dim,dtype", [(8, (1 << 31) - 1, 1024, _lib.F32),      # 2^39 pieces of zeros
+                                                  (100, 100, (1 << 31) - 1, _lib.BF16)])   # slices of the join
+def test_embed_grad_too_large_is_refused_before_any_launch(n, num_rows, dim, dtype):
+    """The call's size is looked at before the sort runs.  (Nothing behind the pointers is touched: here a launch
+    would come back as another error.)"""
+    lib, one = _lib.load(), ctypes.c_void_p(256)
+    rc = lib.hades_embed_grad(one, dim, one, n, one, dim, num_rows, dim, dtype, dtype, _lib.I64, -1, 0, 1.0, 0.0, 0, 0,
+                              ctypes.c_void_p(0), one, 1 << 62, ctypes.c_void_p(0))
+    assert rc == 1 and b"too many values" in lib.hades_last_error()
