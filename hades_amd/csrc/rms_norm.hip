@@ -654,6 +654,8 @@ int hades_rms_norm_grad(const void* grad, int64_t grad_stride, const void* h, in
   HADES_REQUIRE(stream_dtype == dtype || stream_dtype == HADES_F32, "the residual's type is the rows' or float");
   HADES_REQUIRE(weight_dtype == dtype || weight_dtype == HADES_F32, "the weight's type is the rows' or float");
   HADES_REQUIRE(!grad_weight || weight, "grad_weight without a weight");
+  // the partial rows' sum has sixteen threads a column
+  HADES_REQUIRE(!grad_weight || cols <= kMostThreads / kFoldWaves - kWave, "rms_norm_grad: too many columns for one call");
   DropArgs drop;
   HADES_REQUIRE(make_drop(p, seed, offset, offset_ptr, 1.0, &drop), "p must lie in [0, 1]");
   if (rows == 0 && !grad_weight) return HADES_OK;

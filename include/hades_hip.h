@@ -679,7 +679,8 @@ int hades_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_
 
 /* With n = h * rstd and a = grad * weight: grad_res = rstd * (a - n * mean(a * n)) + grad_h (NULL: 0),
  * grad_x = dropout(grad_res), grad_weight = sum over rows of grad * n.  grad_res (stream_dtype) and
- * grad_weight (weight_dtype) may be NULL; workspace is for grad_weight, as for hades_embed_grad. */
+ * grad_weight (weight_dtype) may be NULL; with it cols is at most 2^28 - 64.  workspace is for grad_weight, as for
+ * hades_embed_grad. */
 size_t hades_rms_norm_grad_workspace_bytes(int64_t rows, int64_t cols);
 int hades_rms_norm_grad(const void* grad, int64_t grad_stride, const void* h, int64_t h_stride, const void* weight,
                         const float* rstd, const void* grad_h, int64_t grad_h_stride, void* grad_x, void* grad_res,

@@ -89,3 +89,14 @@ def test_embed_grad_too_large_is_refused_before_any_launch(n, num_rows, dim, dty
     rc = lib.hades_embed_grad(one, dim, one, n, one, dim, num_rows, dim, dtype, dtype, _lib.I64, -1, 0, 1.0, 0.0, 0, 0,
                               ctypes.c_void_p(0), one, 1 << 62, ctypes.c_void_p(0))
     assert rc == 1 and b"too many values" in lib.hades_last_error()
+
+
+def test_rms_norm_grad_of_too_many_columns_is_refused_before_any_launch():
+    lib, one, null = _lib.load(), ctypes.c_void_p(256), ctypes.c_void_p(0)
+
+    def call(rows):
+        return lib.hades_rms_norm_grad(one, cols, one, cols, one, one, null, 0, one, null, one, rows, cols, _lib.BF16,
+                                       _lib.BF16, _lib.BF16, 0.0, 0, 0, null, one, 1 << 62, null)
+    cols = (1 << 28) - 63
+    for rows in (0, 3):
+        assert call(rows) == 1 and b"too many columns" in lib.hades_last_error()
