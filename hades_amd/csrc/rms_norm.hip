@@ -19,7 +19,7 @@
 // a large copy reaches 4.9), into 8 bits with groups of 128 80 - 100 us; gradient with dropout 128 - 150 us (4.5
 // - 5.2 TB/s).  A wave has little work beside its loads, so instructions count: sums and maxima over lanes by
 // data-parallel moves, a reciprocal square root and no division (8 bits, 16 384 x 8 192: 225 instead of 320
-// vector instructions a wave, 173 -> 165 us).  With four pieces a lane (134 registers forward, 277 in the
+// vector instructions a wave, 178 -> 165 us).  With four pieces a lane (134 registers forward, 277 in the
 // gradient) that call took 283 us, and rows of 4 096 206 us in the gradient.
 #include "rowvec.h"
 
@@ -143,11 +143,11 @@ __device__ __forceinline__ float e4m3_scale(uint32_t m) {
 // Eight values in units of `scale`, rounded to e4m3 (nearest even).  scale is the largest magnitude of
 // the group over 448, to half a step: where it is a normal number a value in its units is at most 448 (1 + 2^-22),
 // which rounds to 448, the type's largest.  A subnormal scale of few steps may be too small by a third, and values
-// in its units would reach 672, past the type's range (a NaN); those quotients end at 448.  Quotients by a refined reciprocal and one correction each: of 4 096 x 8 192 bfloat16 values, groups
-// of 128, 2 827 fall to the other side of a tie than in 64 bits; 2 838 with divisions, 3 074 with the reciprocal
-// alone, which takes 170.4 us for 16 384 x 8 192 against 173.  Where the reciprocal would overflow or
-// vanish, or scale is subnormal and coarse, every value is divided; a group of zeros (scale 0), or of magnitudes
-// of up to 224 * 2^-149, whose scale rounds to 0, gives zeros.
+// in its units would reach 672, past the type's range (a NaN); those quotients end at 448.
+// Quotients by a refined reciprocal and one correction each: of 4 096 x 8 192 bfloat16 values, groups of 128, 2 827
+// fall to the other side of a tie than in 64 bits; 2 838 with divisions, 3 074 with the reciprocal alone, which takes
+// 1.5 % less time.  Where the reciprocal would overflow or vanish, or scale is subnormal and coarse, every value is
+// divided; a group of zeros (scale 0), or of magnitudes of up to 224 * 2^-149, whose scale rounds to 0, gives zeros.
 __device__ __forceinline__ void store_e4m3(uint8_t* __restrict__ p, f32x8 v, float scale, int valid) {
   f32x8 u;
   if (scale >= 0x1p-60f && scale < 0x1p100f) {
@@ -655,7 +655,8 @@ int hades_rms_norm_grad(const void* grad, int64_t grad_stride, const void* h, in
   HADES_REQUIRE(weight_dtype == dtype || weight_dtype == HADES_F32, "the weight's type is the rows' or float");
   HADES_REQUIRE(!grad_weight || weight, "grad_weight without a weight");
   // the partial rows' sum has sixteen threads a column
-  HADES_REQUIRE(!grad_weight || cols <= kMostThreads / kFoldWaves - kWave, "rms_norm_grad: too many columns for one call");
+  HADES_REQUIRE(!grad_weight || cols <= kMostThreads / kFoldWaves - kWave,
+                "rms_norm_grad: too many columns for one call");
   DropArgs drop;
   HADES_REQUIRE(make_drop(p, seed, offset, offset_ptr, 1.0, &drop), "p must lie in [0, 1]");
   if (rows == 0 && !grad_weight) return HADES_OK;

@@ -120,7 +120,8 @@ def test_float32_residual_in_training_and_evaluation(cuda_device, dtype, norm):
     h.backward(c)
     masked = ops.dropout(x.detach().float(), *drop)
     assert h.dtype == torch.float32 and torch.equal(h, masked + res)     # the sum's one rounding, in either order
-    assert torch.equal(res.grad, c) and x.grad.dtype == dtype and torch.equal(x.grad, ops.dropout_grad(c, *drop).to(dtype))
+    assert torch.equal(res.grad, c)
+    assert x.grad.dtype == dtype and torch.equal(x.grad, ops.dropout_grad(c, *drop).to(dtype))
     with torch.no_grad():
         again = stage(x, res, offset=drop[2])
         assert torch.equal(again[1] if norm else again, h)
@@ -183,7 +184,7 @@ def test_embed_grad_of_more_than_2_to_29_positions(cuda_device):
     n, vocab, dim = (1 << 29) + 37, 1009, 8
     ids = torch.arange(n, dtype=torch.int32, device="cuda") % vocab
     ids[-5:] = -1
-    rows = torch.arange(8, device="cuda")[:, None] + torch.arange(dim, device="cuda") - 7       # -7 .. 7, by position % 8
+    rows = torch.arange(8, device="cuda")[:, None] + torch.arange(dim, device="cuda") - 7     # -7 .. 7, by position % 8
     grad = rows.to(torch.bfloat16).repeat((n + 7) // 8, 1)[:n]
     got = ops.embed_grad(grad, ids, vocab, out_dtype=torch.float32)
     # the positions of token v: v, v + vocab, ...: eight in a row (vocab is odd) meet each remainder once
