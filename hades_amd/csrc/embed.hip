@@ -22,7 +22,7 @@
 //           token leaves a partial row in every chunk that it touches.  Further blocks of the same
 //           launch write the zeros of the tokens that do not occur.
 //   join    adds the partial rows of the long tokens, in chunk order.
-// 32 768 x 4 096 bfloat16 into 131 072 rows: 236 us for 1.34 GB (5.7 TB/s), of it tokens 6 + 14 (with 80 MiB of the
+// 32 768 x 4 096 bfloat16 into 131 072 rows: 235 us for 1.34 GB (5.7 TB/s), of it tokens 6 + 14 (with 80 MiB of the
 // zeros), sum 203, join 9; 2 048 x 1 024 float32 into 32 000 rows: 31 us for 139 MB, of it tokens 8, sum 19, join 4.
 #include "internal.h"
 #include "rowvec.h"
